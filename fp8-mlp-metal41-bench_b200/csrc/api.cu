@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -679,6 +680,214 @@ int gemm_quantize(int device, int format, const float* src, void* dst, void* sca
   e = launch_quant(format, src, dst, scales, rows, cols, s->num_sms, st);
   if (e != cudaSuccess) return cuda_fail(e, "quantiser launch");
   return GEMM_OK;
+}
+
+}  // extern "C"
+
+// ---- the MLP layer -----------------------------------------------------------------
+// Arguments are checked before the device, so that every refusal shows on a host
+// without a GPU too.
+namespace {
+
+// Makes `device` current and puts the caller's device back.
+struct DeviceScope {
+  int prev = -1;
+  cudaError_t err;
+  explicit DeviceScope(int device) {
+    if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
+    err = prev == device ? cudaSuccess : cudaSetDevice(device);
+    if (prev == device) prev = -1;
+  }
+  ~DeviceScope() {
+    if (prev >= 0) cudaSetDevice(prev);
+  }
+};
+
+constexpr int kMaxDim = 1 << 30;
+
+bool dim_ok(int d) { return d >= 1 && d <= kMaxDim; }
+bool elem_aligned(const void* p, int type) {
+  return (reinterpret_cast<uintptr_t>(p) & (type == kTypeF32 ? 3u : 1u)) == 0;
+}
+long dense(long ld, int cols) { return ld == 0 ? cols : ld; }
+
+// A [rows, cols] operand: present (or optional), aligned to its element, rows apart.
+int check_matrix(const char* name, const void* p, int type, long ld, int cols, bool optional = false) {
+  if (!p) return optional ? GEMM_OK : fail(GEMM_ERR_ARGS, "null %s", name);
+  if (!elem_aligned(p, type)) return fail(GEMM_ERR_ARGS, "%s is not aligned to its element", name);
+  if (dense(ld, cols) < cols) return fail(GEMM_ERR_ARGS, "%s: %ld elements between rows of %d", name, ld, cols);
+  return GEMM_OK;
+}
+
+int make_dropout(const gemm_dropout_args* in, DropArgs* out) {
+  *out = DropArgs();
+  if (!in) return GEMM_OK;
+  if (!(in->p >= 0.0 && in->p <= 1.0)) return fail(GEMM_ERR_ARGS, "dropout probability %g not in 0..1", in->p);
+  if (reinterpret_cast<uintptr_t>(in->offset_ptr) & 7u)
+    return fail(GEMM_ERR_ARGS, "offset_ptr is not 8-byte aligned");
+  out->thr = (uint32_t)std::nearbyint(in->p * 65536.0);
+  out->scale = out->thr < 65536u ? 65536.f / (float)(65536u - out->thr) : 0.f;
+  out->seed = in->seed;
+  out->offset = in->offset;
+  out->offset_ptr = in->offset_ptr;
+  return GEMM_OK;
+}
+
+// The product's operands and sizes from the call's (A, B as stored: X W | dZ W | X dZ).
+LinearArgs product(int op, const void* A, long lda, const void* B, long ldb, int N, int K, int M) {
+  LinearArgs a = {};
+  a.op = op;
+  a.A = A;
+  a.B = B;
+  a.lda = dense(lda, op == kOpDx ? M : K);
+  a.ldb = dense(ldb, M);
+  a.rows = op == kOpDw ? K : N;
+  a.cols = op == kOpDx ? K : M;
+  a.depth = op == kOpLinear ? K : (op == kOpDx ? M : N);
+  return a;
+}
+
+int run_product(int device, LinearArgs& a, int type, int out_type, const char* an, const char* bn, const char* on,
+                void* out, long ldo, int N, int K, int M, const void* res, long ldr, void* ws, size_t ws_bytes,
+                void* stream) {
+  if (type != kTypeF16 && type != kTypeBF16) return fail(GEMM_ERR_ARGS, "operand type %d is not f16 or bf16", type);
+  if (out_type != type && !(a.op == kOpDw && out_type == kTypeF32))
+    return fail(GEMM_ERR_ARGS, "result type %d does not go with operand type %d", out_type, type);
+  if (!dim_ok(N) || !dim_ok(K) || !dim_ok(M))
+    return fail(GEMM_ERR_ARGS, "N=%d K=%d M=%d not in 1..%d", N, K, M, kMaxDim);
+  int rc;
+  if ((rc = check_matrix(an, a.A, type, a.lda, a.op == kOpDx ? M : K))) return rc;
+  if ((rc = check_matrix(bn, a.B, type, a.ldb, M))) return rc;
+  if ((rc = check_matrix(on, out, out_type, ldo, a.cols))) return rc;
+  if ((rc = check_matrix("residual", res, out_type, ldr, a.cols, true))) return rc;
+  a.type = type;
+  a.out_type = out_type;
+  a.out = out;
+  a.ldo = dense(ldo, a.cols);
+  a.res = res;
+  a.ldr = dense(ldr, a.cols);
+  a.ws = ws;
+  a.ws_bytes = ws_bytes;
+  const size_t need = linear_workspace(a);
+  if (need && (!ws || ws_bytes < need)) return fail(GEMM_ERR_ARGS, "workspace of %zu bytes required", need);
+  if (need && (reinterpret_cast<uintptr_t>(ws) & 15u)) return fail(GEMM_ERR_ARGS, "workspace is not 16-byte aligned");
+  DevState* s = dev_state(device);
+  if (!s) return fail(GEMM_ERR_INIT, "device %d not initialised (call gemm_init)", device);
+  a.stream = static_cast<cudaStream_t>(stream);
+  a.dev_err = s->dev_err;
+  a.num_sms = s->num_sms;
+  DeviceScope scope(device);
+  if (scope.err != cudaSuccess) return cuda_fail(scope.err, "cudaSetDevice");
+  const cudaError_t e = launch_linear(a);
+  return e == cudaSuccess ? GEMM_OK : cuda_fail(e, "kernel launch");
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t gemm_linear_workspace(int op, const void* A, long lda, const void* B, long ldb, int N, int K, int M) {
+  if (op < kOpLinear || op > kOpDw || !dim_ok(N) || !dim_ok(K) || !dim_ok(M) || !A || !B) return 0;
+  return linear_workspace(product(op, A, lda, B, ldb, N, K, M));
+}
+
+int gemm_linear(int device, int type, const void* X, long ldx, const void* W, long ldw, void* Y, long ldy, int N,
+                int K, int M, const gemm_epilogue* epi, void* workspace, size_t workspace_bytes, void* stream) {
+  LinearArgs a = product(kOpLinear, X, ldx, W, ldw, N, K, M);
+  const gemm_epilogue none = {};
+  const gemm_epilogue& q = epi ? *epi : none;
+  if (q.act < kActNone || q.act > kActSilu) return fail(GEMM_ERR_ARGS, "unknown activation %d", q.act);
+  int rc;
+  if ((rc = make_dropout(&q.dropout, &a.drop))) return rc;
+  if (q.bias && !elem_aligned(q.bias, type)) return fail(GEMM_ERR_ARGS, "bias is not aligned to its element");
+  if ((rc = check_matrix("preact", q.preact, type, q.ldz, M, true))) return rc;
+  if (q.preact && q.preact == Y) return fail(GEMM_ERR_ARGS, "preact and Y are the same buffer");
+  a.bias = q.bias;
+  a.pre = q.preact;
+  a.ldz = dense(q.ldz, M);
+  a.act = q.act;
+  return run_product(device, a, type, type, "X", "W", "Y", Y, ldy, N, K, M, q.residual, q.ldr, workspace,
+                     workspace_bytes, stream);
+}
+
+int gemm_linear_dx(int device, int type, const void* dZ, long lddz, const void* W, long ldw, void* dX, long lddx,
+                   int N, int K, int M, const void* residual, long ldr, void* workspace, size_t workspace_bytes,
+                   void* stream) {
+  LinearArgs a = product(kOpDx, dZ, lddz, W, ldw, N, K, M);
+  return run_product(device, a, type, type, "dZ", "W", "dX", dX, lddx, N, K, M, residual, ldr, workspace,
+                     workspace_bytes, stream);
+}
+
+int gemm_linear_dw(int device, int type, const void* X, long ldx, const void* dZ, long lddz, void* dW, int out_type,
+                   long lddw, int N, int K, int M, const void* residual, long ldr, void* workspace,
+                   size_t workspace_bytes, void* stream) {
+  LinearArgs a = product(kOpDw, X, ldx, dZ, lddz, N, K, M);
+  return run_product(device, a, type, out_type, "X", "dZ", "dW", dW, lddw, N, K, M, residual, ldr, workspace,
+                     workspace_bytes, stream);
+}
+
+int gemm_act_grad(int device, int type, const void* dY, long lddy, const void* Z, long ldz, void* dZ, long lddz,
+                  float* dbias, int N, int M, int act, const gemm_dropout_args* dropout, void* stream) {
+  if (type != kTypeF16 && type != kTypeBF16) return fail(GEMM_ERR_ARGS, "operand type %d is not f16 or bf16", type);
+  if (!dim_ok(N) || !dim_ok(M)) return fail(GEMM_ERR_ARGS, "N=%d M=%d not in 1..%d", N, M, kMaxDim);
+  if (act < kActNone || act > kActSilu) return fail(GEMM_ERR_ARGS, "unknown activation %d", act);
+  if (!dZ && !dbias) return fail(GEMM_ERR_ARGS, "neither dZ nor dbias given");
+  if (!elem_aligned(dbias, kTypeF32)) return fail(GEMM_ERR_ARGS, "dbias is not aligned to its element");
+  ActGradArgs a = {};
+  int rc;
+  if ((rc = check_matrix("dY", dY, type, lddy, M))) return rc;
+  if ((rc = check_matrix("Z", Z, type, ldz, M, act == kActNone))) return rc;
+  if ((rc = check_matrix("dZ", dZ, type, lddz, M, true))) return rc;
+  if ((rc = make_dropout(dropout, &a.drop))) return rc;
+  a.type = type;
+  a.act = act;
+  a.N = N;
+  a.M = M;
+  a.dY = dY;
+  a.Z = Z;
+  a.dZ = dZ;
+  a.dbias = dbias;
+  a.lddy = dense(lddy, M);
+  a.ldz = dense(ldz, M);
+  a.lddz = dense(lddz, M);
+  DevState* s = dev_state(device);
+  if (!s) return fail(GEMM_ERR_INIT, "device %d not initialised (call gemm_init)", device);
+  a.stream = static_cast<cudaStream_t>(stream);
+  a.num_sms = s->num_sms;
+  DeviceScope scope(device);
+  if (scope.err != cudaSuccess) return cuda_fail(scope.err, "cudaSetDevice");
+  const cudaError_t e = launch_act_grad(a);
+  return e == cudaSuccess ? GEMM_OK : cuda_fail(e, "kernel launch");
+}
+
+int gemm_dropout(int device, int type, const void* X, long ldx, const void* residual, long ldr, void* Y, long ldy,
+                 int N, int M, const gemm_dropout_args* dropout, void* stream) {
+  if (type != kTypeF16 && type != kTypeBF16) return fail(GEMM_ERR_ARGS, "operand type %d is not f16 or bf16", type);
+  if (!dim_ok(N) || !dim_ok(M)) return fail(GEMM_ERR_ARGS, "N=%d M=%d not in 1..%d", N, M, kMaxDim);
+  if (!dropout) return fail(GEMM_ERR_ARGS, "null dropout arguments");
+  DropoutArgs a = {};
+  int rc;
+  if ((rc = check_matrix("X", X, type, ldx, M))) return rc;
+  if ((rc = check_matrix("residual", residual, type, ldr, M, true))) return rc;
+  if ((rc = check_matrix("Y", Y, type, ldy, M))) return rc;
+  if ((rc = make_dropout(dropout, &a.drop))) return rc;
+  a.type = type;
+  a.N = N;
+  a.M = M;
+  a.X = X;
+  a.res = residual;
+  a.Y = Y;
+  a.ldx = dense(ldx, M);
+  a.ldr = dense(ldr, M);
+  a.ldy = dense(ldy, M);
+  DevState* s = dev_state(device);
+  if (!s) return fail(GEMM_ERR_INIT, "device %d not initialised (call gemm_init)", device);
+  a.stream = static_cast<cudaStream_t>(stream);
+  a.num_sms = s->num_sms;
+  DeviceScope scope(device);
+  if (scope.err != cudaSuccess) return cuda_fail(scope.err, "cudaSetDevice");
+  const cudaError_t e = launch_dropout(a);
+  return e == cudaSuccess ? GEMM_OK : cuda_fail(e, "kernel launch");
 }
 
 }  // extern "C"

@@ -84,6 +84,68 @@ void set_last_error(const char* msg);
 cudaError_t launch_quant(int format, const float* src, void* dst, void* scales, long rows, long cols,
                          int num_sms, cudaStream_t st);
 
+// ---- the MLP layer: products with an epilogue, their gradients, dropout --------------
+enum LayerType : int { kTypeF16 = 0, kTypeBF16 = 1, kTypeF32 = 2 };   // GEMM_TYPE_*
+enum LayerAct : int { kActNone = 0, kActRelu = 1, kActGelu = 2, kActGeluTanh = 3, kActSilu = 4 };   // GEMM_ACT_*
+enum LinearOp : int { kOpLinear = 0, kOpDx = 1, kOpDw = 2 };          // GEMM_OP_*
+
+struct DropArgs {
+  uint32_t thr = 0;     // an element is dropped where its 16-bit number is below; 0: no dropout
+  float scale = 1.f;    // 65536 / (65536 - thr); 0 where everything is dropped
+  uint64_t seed = 0, offset = 0;
+  const uint64_t* offset_ptr = nullptr;   // device: added to offset
+};
+
+// One product  out[rows, cols] = R + drop(act(sum_c Row[r, c] Col[c, k] + bias)):
+//   kOpLinear  rows N, cols M, contraction K: Row = X [N,K],         Col = W [K,M]
+//   kOpDx      rows N, cols K, contraction M: Row = dZ [N,M],        Col = W^T, W [K,M]
+//   kOpDw      rows K, cols M, contraction N: Row = X^T, X [N,K],    Col = dZ [N,M]
+struct LinearArgs {
+  int op, type, out_type;
+  const void *A, *B;       // X W | dZ W | X dZ, as stored
+  long lda, ldb;           // elements between their rows
+  int rows, cols, depth;
+  void* out;
+  long ldo;
+  const void* bias;        // [cols] of `type`, or null
+  const void* res;         // [rows, cols] of out_type, or null; may be `out`
+  long ldr;
+  void* pre;               // Z [rows, cols] of `type`, or null
+  long ldz;
+  int act;
+  DropArgs drop;
+  void* ws;
+  size_t ws_bytes;
+  cudaStream_t stream;
+  int* dev_err;
+  int num_sms;
+};
+size_t linear_workspace(const LinearArgs& a);
+cudaError_t launch_linear(const LinearArgs& a);
+
+struct ActGradArgs {
+  int type, act, N, M;
+  const void *dY, *Z;
+  void* dZ;                // may be null (the column sums alone)
+  float* dbias;            // may be null
+  long lddy, ldz, lddz;
+  DropArgs drop;
+  cudaStream_t stream;
+  int num_sms;
+};
+cudaError_t launch_act_grad(const ActGradArgs& a);
+
+struct DropoutArgs {
+  int type, N, M;
+  const void *X, *res;
+  void* Y;
+  long ldx, ldr, ldy;
+  DropArgs drop;
+  cudaStream_t stream;
+  int num_sms;
+};
+cudaError_t launch_dropout(const DropoutArgs& a);
+
 // ---- peak probe -----------------------------------------------------------------
 cudaError_t launch_peak(int kind, int reps, int ctas, float* sink, int* dev_err,
                         cudaStream_t st);

@@ -26,6 +26,7 @@ EXPORTS = [
     "gemm_read_probe",
     "gemm_run_noalloc",
     "gemm_quantize",
+    "gemm_linear", "gemm_linear_dx", "gemm_linear_dw", "gemm_linear_workspace", "gemm_act_grad", "gemm_dropout",
     "gemm_run_gather", "gemm_gather_supported", "gemm_peer_alloc", "gemm_peer_open", "gemm_peer_close",
 ]
 
@@ -34,6 +35,24 @@ PEER_HANDLE_BYTES = 64   # GEMM_PEER_HANDLE_BYTES
 
 # quantiser formats (GEMM_Q_* in include/mlpgemm.h)
 Q_E4M3_REF, Q_E4M3, Q_E2M1, Q_MXFP4, Q_MXFP8 = 0, 1, 2, 3, 4
+
+# the MLP layer's operand types (GEMM_TYPE_*), activations (GEMM_ACT_*) and products (GEMM_OP_*)
+TYPES = {"f16": 0, "bf16": 1, "f32": 2}
+ACTS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+OP_LINEAR, OP_DX, OP_DW = 0, 1, 2
+
+
+class DropoutArgs(ctypes.Structure):
+    """gemm_dropout_args"""
+    _fields_ = [("p", ctypes.c_double), ("seed", ctypes.c_uint64), ("offset", ctypes.c_uint64),
+                ("offset_ptr", ctypes.c_void_p)]
+
+
+class Epilogue(ctypes.Structure):
+    """gemm_epilogue"""
+    _fields_ = [("bias", ctypes.c_void_p), ("residual", ctypes.c_void_p), ("ldr", ctypes.c_long),
+                ("preact", ctypes.c_void_p), ("ldz", ctypes.c_long), ("act", ctypes.c_int),
+                ("dropout", DropoutArgs)]
 
 
 class GemmError(RuntimeError):
@@ -54,6 +73,7 @@ def build() -> str:
 
 def _declare(L):
     c_int, c_size, vp, c_char_p = ctypes.c_int, ctypes.c_size_t, ctypes.c_void_p, ctypes.c_char_p
+    c_long = ctypes.c_long
     vpp = ctypes.POINTER(ctypes.c_void_p)
     sig = {
         "gemm_init": (c_int, [c_int]),
@@ -96,6 +116,16 @@ def _declare(L):
         "gemm_run_noalloc": (c_int, [c_int, c_int, c_int, vp, vp, vp, c_int, c_int, c_int, vp, vp,
                                      vp]),
         "gemm_quantize": (c_int, [c_int, c_int, vp, vp, vp, ctypes.c_long, ctypes.c_long, vp]),
+        "gemm_linear": (c_int, [c_int, c_int, vp, c_long, vp, c_long, vp, c_long, c_int, c_int, c_int, vp, vp,
+                                c_size, vp]),
+        "gemm_linear_dx": (c_int, [c_int, c_int, vp, c_long, vp, c_long, vp, c_long, c_int, c_int, c_int, vp,
+                                   c_long, vp, c_size, vp]),
+        "gemm_linear_dw": (c_int, [c_int, c_int, vp, c_long, vp, c_long, vp, c_int, c_long, c_int, c_int, c_int,
+                                   vp, c_long, vp, c_size, vp]),
+        "gemm_linear_workspace": (c_size, [c_int, vp, c_long, vp, c_long, c_int, c_int, c_int]),
+        "gemm_act_grad": (c_int, [c_int, c_int, vp, c_long, vp, c_long, vp, c_long, vp, c_int, c_int, c_int, vp,
+                                  vp]),
+        "gemm_dropout": (c_int, [c_int, c_int, vp, c_long, vp, c_long, vp, c_long, c_int, c_int, vp, vp]),
         "gemm_run_gather": (c_int, [c_int, c_int, c_int, vp, vp, vp, c_int, c_int, c_int, vp, vp, vp,
                                     c_size, vpp, c_int, vp]),
         "gemm_gather_supported": (c_int, [c_int, c_int]),
@@ -358,3 +388,56 @@ def quantize(device, fmt, src, dst, scales=None, rows=1, cols=1, stream=None) ->
     """f32 [rows, cols] on the device -> a GEMM_Q_* format in `dst` (+ UE8M0 `scales`)."""
     check(lib().gemm_quantize(device, fmt, as_ptr(src), as_ptr(dst), as_ptr(scales), int(rows), int(cols),
                               as_ptr(stream)), "gemm_quantize")
+
+
+# ---- the MLP layer (f16 / bf16 operands; see the header for the formulas) -----------------
+def _dropout(p, seed, offset, offset_ptr) -> DropoutArgs:
+    return DropoutArgs(p, seed, offset, as_ptr(offset_ptr))
+
+
+def linear_workspace(op: int, A, B, N: int, K: int, M: int, lda: int = 0, ldb: int = 0) -> int:
+    """Workspace bytes of a product: A, B are X, W (OP_LINEAR), dZ, W (OP_DX) or X, dZ (OP_DW)."""
+    return lib().gemm_linear_workspace(op, as_ptr(A), lda, as_ptr(B), ldb, N, K, M)
+
+
+def linear(device, type, X, W, Y, N, K, M, bias=None, act=0, residual=None, preact=None, dropout_p=0.0, seed=0,
+           offset=0, offset_ptr=None, ldx=0, ldw=0, ldy=0, ldr=0, ldz=0, workspace=None, workspace_bytes=0,
+           stream=None) -> None:
+    """Y = residual + dropout(act(X @ W + bias)); preact receives X @ W + bias.  Row lengths 0: dense."""
+    epi = Epilogue(as_ptr(bias), as_ptr(residual), ldr, as_ptr(preact), ldz, act,
+                   _dropout(dropout_p, seed, offset, offset_ptr))
+    check(lib().gemm_linear(device, type, as_ptr(X), ldx, as_ptr(W), ldw, as_ptr(Y), ldy, N, K, M,
+                            ctypes.addressof(epi), as_ptr(workspace), int(workspace_bytes), as_ptr(stream)),
+          "gemm_linear")
+
+
+def linear_dx(device, type, dZ, W, dX, N, K, M, residual=None, lddz=0, ldw=0, lddx=0, ldr=0, workspace=None,
+              workspace_bytes=0, stream=None) -> None:
+    """dX = residual + dZ @ W^T."""
+    check(lib().gemm_linear_dx(device, type, as_ptr(dZ), lddz, as_ptr(W), ldw, as_ptr(dX), lddx, N, K, M,
+                               as_ptr(residual), ldr, as_ptr(workspace), int(workspace_bytes), as_ptr(stream)),
+          "gemm_linear_dx")
+
+
+def linear_dw(device, type, X, dZ, dW, N, K, M, out_type=None, residual=None, ldx=0, lddz=0, lddw=0, ldr=0,
+              workspace=None, workspace_bytes=0, stream=None) -> None:
+    """dW = residual + X^T @ dZ, of `out_type` (default: the operands' type)."""
+    check(lib().gemm_linear_dw(device, type, as_ptr(X), ldx, as_ptr(dZ), lddz, as_ptr(dW),
+                               type if out_type is None else out_type, lddw, N, K, M, as_ptr(residual), ldr,
+                               as_ptr(workspace), int(workspace_bytes), as_ptr(stream)), "gemm_linear_dw")
+
+
+def act_grad(device, type, dY, Z, dZ, dbias, N, M, act=0, dropout_p=0.0, seed=0, offset=0, offset_ptr=None,
+             lddy=0, ldz=0, lddz=0, stream=None) -> None:
+    """dZ = dropout(dY) * act'(Z); dbias (f32) = its column sums."""
+    drop = _dropout(dropout_p, seed, offset, offset_ptr)
+    check(lib().gemm_act_grad(device, type, as_ptr(dY), lddy, as_ptr(Z), ldz, as_ptr(dZ), lddz, as_ptr(dbias), N, M,
+                              act, ctypes.addressof(drop), as_ptr(stream)), "gemm_act_grad")
+
+
+def dropout(device, type, X, Y, N, M, p, seed, offset, offset_ptr=None, residual=None, ldx=0, ldr=0, ldy=0,
+            stream=None) -> None:
+    """Y = residual + dropout(X); on dY the same call is its gradient."""
+    drop = _dropout(p, seed, offset, offset_ptr)
+    check(lib().gemm_dropout(device, type, as_ptr(X), ldx, as_ptr(residual), ldr, as_ptr(Y), ldy, N, M,
+                             ctypes.addressof(drop), as_ptr(stream)), "gemm_dropout")

@@ -286,6 +286,100 @@ int gemm_read_probe(int device, const void *buf, size_t bytes, int warmup, int i
 int gemm_quantize(int device, int format, const float *src, void *dst, void *scales,
                   long rows, long cols, void *stream);
 
+/* ---- the MLP layer: the product with its epilogue, its gradients, dropout --------
+ * The reference stops at the bare product; a layer that is served or trained
+ * needs what follows.  Operands are IEEE half or bfloat16 (`type`, the same for
+ * every operand of a call), row-major with `ld*` elements between rows (0: dense;
+ * else at least the row's length).  Sums are f32 and each result is rounded once,
+ * to nearest even.
+ *
+ *   gemm_linear     Y[N,M]  = R + D(act(X[N,K] @ W[K,M] + bias))
+ *                   Z[N,M]  = X @ W + bias, stored where `preact` is given
+ *   gemm_linear_dx  dX[N,K] = R + dZ[N,M] @ W[K,M]^T
+ *   gemm_linear_dw  dW[K,M] = R + X[N,K]^T @ dZ[N,M]
+ *   gemm_act_grad   dZ[N,M] = D(dY) * act'(Z);  dbias[M] = its column sums (f32,
+ *                   of the values before dZ is rounded)
+ *   gemm_dropout    Y[N,M]  = R + D(X); its gradient is the same call on dY
+ *
+ * A training step of  Y = R + D(act(X W + b))  is gemm_linear with `preact`, then
+ * gemm_act_grad (dZ, dbias), gemm_linear_dx and gemm_linear_dw; R's gradient is dY.
+ *
+ * D is dropout with probability p, its mask computed and never stored.  Element
+ * (r, c) of the call's output is dropped (0, whatever it held) where a 16-bit
+ * number u(r, c) is below t = rint(65536 p), else multiplied by 65536 / (65536 - t);
+ * p = 0 switches D off, p = 1 drops everything.  u comes from Philox4x32-10 with
+ * the seed's words as the key and the counter (c / 8, r, offset's low word, high
+ * word): half-word c % 8 of its 128 bits, low halves first.  The mask depends on
+ * nothing else, so forward and backward agree whatever kernel computes them.
+ * Give every layer and step another offset.  `offset_ptr`, if not NULL, is a
+ * device word that is read when the call runs and added to `offset`: a captured
+ * graph gets new masks from replay to replay by writing it in between.
+ *
+ * R (`residual`) has the result's type and may be the result's buffer itself (the
+ * same pointer and row length); no other input may overlap an output.  Elements
+ * between a row's end and the next row are neither read nor written.
+ * N, K, M are 1 .. 2^30.  Pointers are aligned to their element.  Any size,
+ * stride and alignment works; X, W and dZ are read in place where their base and
+ * rows are 16-byte aligned, and are laid out in the workspace first where not
+ * (gemm_linear_workspace; 0 for aligned operands).  The workspace needs no
+ * initialisation and may be reused by the next call on the stream; calls that
+ * may overlap need one each.
+ * Asynchronous on `stream` (NULL = the default stream), without allocation or
+ * synchronisation, so capturable; the caller's current device is the same on
+ * return.  A call with an argument error enqueues nothing. */
+#define GEMM_TYPE_F16  0
+#define GEMM_TYPE_BF16 1
+#define GEMM_TYPE_F32  2    /* dW only */
+
+#define GEMM_ACT_NONE      0
+#define GEMM_ACT_RELU      1    /* slope 0 at 0 */
+#define GEMM_ACT_GELU      2    /* z Phi(z) */
+#define GEMM_ACT_GELU_TANH 3    /* 0.5 z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) */
+#define GEMM_ACT_SILU      4    /* z / (1 + exp(-z)) */
+
+typedef struct gemm_dropout_args {
+  double p;                     /* 0 .. 1 */
+  uint64_t seed, offset;
+  const uint64_t *offset_ptr;   /* device memory, or NULL */
+} gemm_dropout_args;
+
+typedef struct gemm_epilogue {
+  const void *bias;             /* [M] of `type`, or NULL */
+  const void *residual;         /* [N,M] of `type`, or NULL */
+  long ldr;
+  void *preact;                 /* [N,M] of `type`, or NULL */
+  long ldz;
+  int act;                      /* GEMM_ACT_* */
+  gemm_dropout_args dropout;
+} gemm_epilogue;
+
+/* `epi` NULL: Y = X @ W. */
+int gemm_linear(int device, int type, const void *X, long ldx, const void *W, long ldw, void *Y, long ldy,
+                int N, int K, int M, const gemm_epilogue *epi, void *workspace, size_t workspace_bytes,
+                void *stream);
+int gemm_linear_dx(int device, int type, const void *dZ, long lddz, const void *W, long ldw, void *dX, long lddx,
+                   int N, int K, int M, const void *residual, long ldr, void *workspace, size_t workspace_bytes,
+                   void *stream);
+/* dW and its residual are of `out_type`: `type`, or GEMM_TYPE_F32 (gradients
+ * accumulated over micro-batches: residual = dW). */
+int gemm_linear_dw(int device, int type, const void *X, long ldx, const void *dZ, long lddz, void *dW,
+                   int out_type, long lddw, int N, int K, int M, const void *residual, long ldr,
+                   void *workspace, size_t workspace_bytes, void *stream);
+/* Workspace bytes of a product with these operands: A, B as the call takes them
+ * (X, W; dZ, W; X, dZ), 0 for arguments that the call refuses. */
+#define GEMM_OP_LINEAR 0
+#define GEMM_OP_DX     1
+#define GEMM_OP_DW     2
+size_t gemm_linear_workspace(int op, const void *A, long lda, const void *B, long ldb, int N, int K, int M);
+
+/* Z may be NULL with GEMM_ACT_NONE; either of dZ and dbias may be NULL; dZ may be
+ * dY's or Z's buffer itself (the same pointer and row length).  `dropout` NULL: none. */
+int gemm_act_grad(int device, int type, const void *dY, long lddy, const void *Z, long ldz, void *dZ, long lddz,
+                  float *dbias, int N, int M, int act, const gemm_dropout_args *dropout, void *stream);
+/* Y may also be X's buffer itself. */
+int gemm_dropout(int device, int type, const void *X, long ldx, const void *residual, long ldr, void *Y, long ldy,
+                 int N, int M, const gemm_dropout_args *dropout, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
