@@ -54,6 +54,29 @@ __device__ __forceinline__ float act_fwd(float z, int act) {
   }
 }
 
+// The same for eight values: one branch on the activation, not eight.
+__device__ __forceinline__ void act_fwd8(float (&v)[8], int act) {
+  switch (act) {
+    case kActRelu:
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = act_fwd(v[i], kActRelu);
+      break;
+    case kActGelu:
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = act_fwd(v[i], kActGelu);
+      break;
+    case kActGeluTanh:
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = act_fwd(v[i], kActGeluTanh);
+      break;
+    case kActSilu:
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = act_fwd(v[i], kActSilu);
+      break;
+    default: break;
+  }
+}
+
 // act'(z).  z is a stored pre-activation, which f16 may have rounded to an
 // infinity: beyond the clamps every slope is 0 or 1 to f32 precision, so an
 // infinite z gets its limit instead of inf * 0.  NaN passes the comparisons.

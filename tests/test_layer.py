@@ -177,7 +177,7 @@ def linear_ref(x, w, bias, res, act, p, seed, offset):
 
 SIZES = [(1, 1, 1), (1, 64, 8), (2, 4096, 264), (3, 7, 5), (13, 520, 1000), (16, 129, 24), (17, 100, 33),
          (40, 64, 136), (65, 72, 257), (128, 512, 256), (130, 257, 264), (200, 1000, 520), (257, 640, 1032),
-         (700, 96, 2056), (1100, 520, 1288)]
+         (700, 96, 2056), (1100, 520, 1288), (1300, 136, 2056), (1030, 77, 2571), (2310, 1160, 1112), (4200, 64, 808)]
 
 
 @pytest.mark.gpu
@@ -205,11 +205,11 @@ def test_linear_sizes(gemm, size, type):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("act", ACT_NAMES)
-@pytest.mark.parametrize("N", [5, 300])
+@pytest.mark.parametrize("N,M", [(5, 328), (300, 328), (1300, 2056)])
 @pytest.mark.parametrize("bias,res,pre,p", [(1, 0, 0, 0.0), (0, 1, 0, 0.0), (0, 0, 1, 0.0), (0, 0, 0, 0.5),
                                             (0, 1, 1, 1.0), (1, 1, 1, 0.1)])
-def test_linear_epilogues(gemm, act, N, bias, res, pre, p):
-    K, M, t = 200, 328, torch.bfloat16
+def test_linear_epilogues(gemm, act, N, M, bias, res, pre, p):
+    K, t = 200, torch.bfloat16
     x, w = rand((N, K), t, 1, 2.0), rand((K, M), t, 2, K ** -0.5)
     b = rand((M,), t, 3) if bias else None
     r = rand((N, M), t, 4) if res else None
@@ -227,17 +227,18 @@ def test_linear_epilogues(gemm, act, N, bias, res, pre, p):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("N", [1, 13, 140, 600])
+@pytest.mark.parametrize("N,M", [(1, 200), (13, 200), (140, 200), (600, 200), (1290, 2000)])
 @pytest.mark.parametrize("pad,shift", [(8, 8), (3, 1), (0, 1)])
-def test_linear_strides_and_alignment(gemm, N, pad, shift):
+def test_linear_strides_and_alignment(gemm, N, M, pad, shift):
     # rows further apart than their length, buffers that start anywhere; the gaps keep what they held
-    K, M, t = 136, 200, torch.float16
+    K, t = 136, torch.float16
     x0, w0, b, r0 = rand((N, K), t, 1), rand((K, M), t, 2, K ** -0.5), rand((M,), t, 3), rand((N, M), t, 4)
     x, w, r = put(x0, K + pad, shift), put(w0, M + pad, shift), put(r0, M + pad, shift)
     b1 = torch.cat([b[:1], b])[1:]                      # two bytes past an aligned address
     ybuf, y = strided((N, M), t, M + pad, shift, 7.0)
     zbuf, z = strided((N, M), t, M + pad, shift, 7.0)
     ws, wsb = workspace(G.OP_LINEAR, x, w, N, K, M, K + pad, M + pad)
+    assert (wsb == 0) == (shift == 8)
     G.linear(0, G.TYPES["f16"], x, w, y, N, K, M, bias=b1, act=G.ACTS["gelu"], residual=r, preact=z, dropout_p=0.2,
              seed=9, offset=1, ldx=K + pad, ldw=M + pad, ldy=M + pad, ldr=M + pad, ldz=M + pad, workspace=ws,
              workspace_bytes=wsb, stream=stream())
@@ -251,9 +252,9 @@ def test_linear_strides_and_alignment(gemm, N, pad, shift):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("N", [4, 333])
-def test_linear_residual_in_place(gemm, N):
-    K, M, t = 264, 272, torch.bfloat16
+@pytest.mark.parametrize("N,M", [(4, 272), (333, 272), (1300, 2056)])
+def test_linear_residual_in_place(gemm, N, M):
+    K, t = 264, torch.bfloat16
     x, w, r = rand((N, K), t, 1), rand((K, M), t, 2, K ** -0.5), rand((N, M), t, 4)
     y = r.clone()
     G.linear(0, G.TYPES["bf16"], x, w, y, N, K, M, residual=y, stream=stream())
@@ -263,10 +264,10 @@ def test_linear_residual_in_place(gemm, N):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("N", [7, 260])
-def test_linear_specials_stay_in_their_rows(gemm, N):
+@pytest.mark.parametrize("N,M", [(7, 264), (260, 264), (1300, 2056)])
+def test_linear_specials_stay_in_their_rows(gemm, N, M):
     # an infinity or NaN in X reaches its own row alone; a dropped element is 0 whatever it held
-    K, M, t = 72, 264, torch.float16
+    K, t = 72, torch.float16
     x, w = rand((N, K), t, 1), rand((K, M), t, 2, K ** -0.5)
     x[2, 3], x[4, 0] = float("nan"), float("inf")
     y = torch.empty(N, M, dtype=t, device="cuda")
@@ -283,7 +284,7 @@ def test_linear_specials_stay_in_their_rows(gemm, N):
 
 
 GRAD_SIZES = [(1, 1, 1), (1, 264, 136), (5, 9, 7), (16, 520, 1032), (33, 257, 129), (64, 128, 128), (130, 1000, 264),
-              (333, 136, 2056), (600, 520, 520), (1050, 72, 200), (2100, 256, 264)]
+              (333, 136, 2056), (600, 520, 520), (1050, 72, 200), (2100, 256, 264), (1300, 2056, 1288), (1029, 2571, 1101), (520, 2312, 1544), (65, 2600, 2056)]
 
 
 @pytest.mark.gpu
@@ -316,7 +317,7 @@ def test_gradient_products(gemm, size, type):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("size", [(13, 136, 200), (300, 200, 136)], ids=str)
+@pytest.mark.parametrize("size", [(13, 136, 200), (300, 200, 136), (1300, 2056, 1800)], ids=str)
 @pytest.mark.parametrize("pad,shift", [(8, 8), (3, 1)])
 def test_gradient_products_strided(gemm, size, pad, shift):
     (N, K, M), t = size, torch.bfloat16
@@ -344,6 +345,19 @@ def test_gradient_products_strided(gemm, size, pad, shift):
         assert_close(dw, v, product_error(x0.t(), dz0, N) + v.abs() * 2.0 ** -23 + half_step(v, o) * 1.01, "dW")
         dw.fill_(7.0)
         assert bool((buf == 7.0).all())
+
+
+@pytest.mark.gpu
+def test_dw_long_sum_in_32_bits(gemm):
+    # accumulated over many rows, the f32 gradient stays within 1e-6 of the 64-bit sum (2-norm): partial sums of
+    # 512 rows leave the tensor cores, whose adds cut, before 512/16 of them have lost 32 * 2^-25 = 1e-6
+    N, K, M = 8192, 264, 512
+    x, dz = rand((N, K), torch.bfloat16, 1), rand((N, M), torch.bfloat16, 2)
+    dw = torch.empty(K, M, device="cuda")
+    G.linear_dw(0, G.TYPES["bf16"], x, dz, dw, N, K, M, out_type=G.TYPES["f32"], stream=stream())
+    G.sync(0, stream())
+    ref = x.double().t() @ dz.double()
+    assert float((dw.double() - ref).norm() / ref.norm()) <= 1e-6
 
 
 # ---- the epilogue's gradient ----------------------------------------------------------------
@@ -630,6 +644,19 @@ def test_good_arguments_need_the_device():
         with pytest.raises(G.GemmError) as e:
             call()
         assert e.value.code == G.GEMM_ERR_INIT
+
+
+def test_workspace_is_for_operands_the_tma_cannot_read():
+    ws = G.linear_workspace
+    assert ws(G.OP_LINEAR, P, P, 128, 1024, 2048) == 0
+    assert ws(G.OP_LINEAR, P, P, 128, 1000, 2048, 1008, 2048) == 0
+    assert ws(G.OP_LINEAR, P, P, 128, 1001, 2048) >= 128 * 1001 * 2          # X's rows
+    assert ws(G.OP_LINEAR, P, P + 2, 128, 1024, 2048) >= 1024 * 2048 * 2     # W's base
+    assert ws(G.OP_DX, P, P, 128, 1024, 1001) >= 128 * 1001 * 2 + 1024 * 1001 * 2
+    assert ws(G.OP_DW, P, P, 128, 1001, 1024) >= 128 * 1001 * 2
+    assert ws(G.OP_DW, P, P, 128, 1001, 1024, 1001, 0) < 128 * 1002 * 2 + 4096
+    assert ws(3, P, P, 128, 1024, 2048) == 0 and ws(G.OP_LINEAR, None, P, 128, 1001, 2048) == 0
+    assert ws(G.OP_LINEAR, P, P, 0, 1001, 2048) == 0
 
 
 def test_structures_match_the_header():
