@@ -10,31 +10,77 @@
 namespace mlpg {
 
 // ---- 16-bit types ----------------------------------------------------------------
+// The type is a template parameter (kTypeF16, kTypeBF16): a branch per conversion cost
+// the epilogues more than the conversion.
+
 // Two values of a 32-bit word, low half first.
-__device__ __forceinline__ float2 unpack2(uint32_t w, int type) {
-  if (type == kTypeF16) return __half22float2(*reinterpret_cast<const __half2*>(&w));
-  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+template <int TYPE>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if constexpr (TYPE == kTypeF16) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
 }
 
 // Round to nearest even, both types; f16 overflows to infinity.
-__device__ __forceinline__ uint32_t pack2(float lo, float hi, int type) {
-  if (type == kTypeF16) {
+template <int TYPE>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (TYPE == kTypeF16) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&b);
   }
-  const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&b);
 }
 
-__device__ __forceinline__ float load1(const void* base, size_t i, int type) {
-  if (type == kTypeF32) return static_cast<const float*>(base)[i];
-  const uint32_t w = static_cast<const uint16_t*>(base)[i];
-  return unpack2(w, type).x;
+template <int TYPE>
+__device__ __forceinline__ float load1(const void* base, size_t i) {
+  return unpack2<TYPE>(static_cast<const uint16_t*>(base)[i]).x;
 }
 
-__device__ __forceinline__ void store1(void* base, size_t i, float v, int type) {
-  if (type == kTypeF32) static_cast<float*>(base)[i] = v;
-  else static_cast<uint16_t*>(base)[i] = (uint16_t)(pack2(v, 0.f, type) & 0xFFFFu);
+template <int TYPE>
+__device__ __forceinline__ void store1(void* base, size_t i, float v) {
+  static_cast<uint16_t*>(base)[i] = (uint16_t)(pack2<TYPE>(v, 0.f) & 0xFFFFu);
+}
+
+// Eight neighbours in 16 bytes.
+template <int TYPE>
+__device__ __forceinline__ void unpack8(float (&v)[8], uint4 w) {
+  const uint32_t q[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = unpack2<TYPE>(q[i]);
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+
+template <int TYPE>
+__device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
+  return make_uint4(pack2<TYPE>(v[0], v[1]), pack2<TYPE>(v[2], v[3]), pack2<TYPE>(v[4], v[5]),
+                    pack2<TYPE>(v[6], v[7]));
+}
+
+// Eight elements of a row of `cols` from column c on, element `at` of base: one 16-byte
+// access where the rows allow it (vec); elements past the row read as 0 and are not written.
+template <int TYPE>
+__device__ __forceinline__ void load8(float (&v)[8], const void* base, size_t at, int c, int cols, bool vec) {
+  if (vec && c + 8 <= cols) {
+    unpack8<TYPE>(v, *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + at));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? load1<TYPE>(base, at + i) : 0.f;
+  }
+}
+
+template <int TYPE>
+__device__ __forceinline__ void store8(const float (&v)[8], void* base, size_t at, int c, int cols, bool vec) {
+  if (vec && c + 8 <= cols) {
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + at) = pack8<TYPE>(v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (c + i < cols) store1<TYPE>(base, at + i, v[i]);
+  }
 }
 
 // ---- activations ------------------------------------------------------------------
@@ -44,34 +90,47 @@ __device__ __forceinline__ float sigmoidf_(float t) { return __fdividef(1.f, 1.f
 
 __device__ __forceinline__ float gelu_u2(float z) { return 1.5957691216057308f * (z + 0.044715f * z * z * z); }
 
-__device__ __forceinline__ float act_fwd(float z, int act) {
-  switch (act) {
-    case kActRelu: return z < 0.f ? 0.f : z;   // NaN stays NaN
-    case kActGelu: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
-    case kActGeluTanh: return z * sigmoidf_(gelu_u2(z));
-    case kActSilu: return z * sigmoidf_(z);
-    default: return z;
-  }
+// Phi(z), the normal distribution, and e = exp(-z^2/2) by Abramowitz and Stegun 7.1.26:
+// erfc(x) = (a1 t + ... + a5 t^5) exp(-x^2), t = 1 / (1 + 0.3275911 x), off by at most
+// 1.5e-7: far below a 16-bit result's rounding, no branch, and the slope reuses e.
+__device__ __forceinline__ float normal_cdf(float z, float& e) {
+  const float t = __fdividef(1.f, 1.f + 0.23164189f * fabsf(z));   // 0.3275911 / sqrt(2)
+  e = __expf(-0.5f * z * z);
+  const float poly = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+  const float tail = 0.5f * poly * e;
+  return z < 0.f ? tail : 1.f - tail;
 }
 
-// The same for eight values: one branch on the activation, not eight.
+template <int ACT>
+__device__ __forceinline__ float act_fwd(float z) {
+  if constexpr (ACT == kActRelu) return z < 0.f ? 0.f : z;   // NaN stays NaN
+  if constexpr (ACT == kActGelu) {
+    float e;
+    return z * normal_cdf(z, e);
+  }
+  if constexpr (ACT == kActGeluTanh) return z * sigmoidf_(gelu_u2(z));
+  if constexpr (ACT == kActSilu) return z * sigmoidf_(z);
+  return z;
+}
+
+// The same for eight values and an activation known at run time: one branch for all.
 __device__ __forceinline__ void act_fwd8(float (&v)[8], int act) {
   switch (act) {
     case kActRelu:
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = act_fwd(v[i], kActRelu);
+      for (int i = 0; i < 8; ++i) v[i] = act_fwd<kActRelu>(v[i]);
       break;
     case kActGelu:
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = act_fwd(v[i], kActGelu);
+      for (int i = 0; i < 8; ++i) v[i] = act_fwd<kActGelu>(v[i]);
       break;
     case kActGeluTanh:
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = act_fwd(v[i], kActGeluTanh);
+      for (int i = 0; i < 8; ++i) v[i] = act_fwd<kActGeluTanh>(v[i]);
       break;
     case kActSilu:
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = act_fwd(v[i], kActSilu);
+      for (int i = 0; i < 8; ++i) v[i] = act_fwd<kActSilu>(v[i]);
       break;
     default: break;
   }
@@ -80,25 +139,26 @@ __device__ __forceinline__ void act_fwd8(float (&v)[8], int act) {
 // act'(z).  z is a stored pre-activation, which f16 may have rounded to an
 // infinity: beyond the clamps every slope is 0 or 1 to f32 precision, so an
 // infinite z gets its limit instead of inf * 0.  NaN passes the comparisons.
-__device__ __forceinline__ float act_slope(float z, int act) {
-  switch (act) {
-    case kActRelu: return z > 0.f ? 1.f : (z <= 0.f ? 0.f : z);
-    case kActGelu: {
-      z = z > 30.f ? 30.f : (z < -30.f ? -30.f : z);
-      return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * __expf(-0.5f * z * z) * 0.3989422804014327f;
-    }
-    case kActGeluTanh: {
-      z = z > 30.f ? 30.f : (z < -30.f ? -30.f : z);
-      const float q = sigmoidf_(gelu_u2(z));
-      return q + z * q * (1.f - q) * (1.5957691216057308f * (1.f + 0.134145f * z * z));
-    }
-    case kActSilu: {
-      z = z > 80.f ? 80.f : (z < -80.f ? -80.f : z);
-      const float q = sigmoidf_(z);
-      return q * (1.f + z * (1.f - q));
-    }
-    default: return 1.f;
+template <int ACT>
+__device__ __forceinline__ float act_slope(float z) {
+  if constexpr (ACT == kActRelu) return z > 0.f ? 1.f : (z <= 0.f ? 0.f : z);
+  if constexpr (ACT == kActGelu) {
+    z = z > 30.f ? 30.f : (z < -30.f ? -30.f : z);
+    float e;
+    const float phi = normal_cdf(z, e);
+    return phi + z * e * 0.3989422804014327f;
   }
+  if constexpr (ACT == kActGeluTanh) {
+    z = z > 30.f ? 30.f : (z < -30.f ? -30.f : z);
+    const float q = sigmoidf_(gelu_u2(z));
+    return q + z * q * (1.f - q) * (1.5957691216057308f * (1.f + 0.134145f * z * z));
+  }
+  if constexpr (ACT == kActSilu) {
+    z = z > 80.f ? 80.f : (z < -80.f ? -80.f : z);
+    const float q = sigmoidf_(z);
+    return q * (1.f + z * (1.f - q));
+  }
+  return 1.f;
 }
 
 // ---- dropout ------------------------------------------------------------------------
@@ -144,14 +204,6 @@ __device__ __forceinline__ void drop8(float (&v)[8], const DropArgs& d, uint64_t
     v[2 * i] = (w[i] & 0xFFFFu) >= d.thr ? v[2 * i] * d.scale : 0.f;
     v[2 * i + 1] = (w[i] >> 16) >= d.thr ? v[2 * i + 1] * d.scale : 0.f;
   }
-}
-
-__device__ __forceinline__ float drop1(float v, const DropArgs& d, uint64_t off, int row, int col) {
-  const uint4 b = drop_bits(d, off, row, col >> 3);
-  const uint32_t w[4] = {b.x, b.y, b.z, b.w};
-  const int i = col & 7;
-  const uint32_t u = (w[i >> 1] >> (16 * (i & 1))) & 0xFFFFu;
-  return u >= d.thr ? v * d.scale : 0.f;
 }
 
 }  // namespace mlpg
