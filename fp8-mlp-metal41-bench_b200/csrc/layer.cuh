@@ -60,26 +60,35 @@ __device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
                     pack2<TYPE>(v[6], v[7]));
 }
 
-// Eight elements of a row of `cols` from column c on, element `at` of base: one 16-byte
+// W (4 or 8) elements of a row of `cols` from column c on, element `at` of base: one
 // access where the rows allow it (vec); elements past the row read as 0 and are not written.
-template <int TYPE>
-__device__ __forceinline__ void load8(float (&v)[8], const void* base, size_t at, int c, int cols, bool vec) {
-  if (vec && c + 8 <= cols) {
-    unpack8<TYPE>(v, *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + at));
+template <int TYPE, int W>
+__device__ __forceinline__ void loadn(float (&v)[W], const void* base, size_t at, int c, int cols, bool vec) {
+  const uint16_t* p = static_cast<const uint16_t*>(base) + at;
+  if (vec && c + W <= cols) {
+    if constexpr (W == 8) {
+      unpack8<TYPE>(v, *reinterpret_cast<const uint4*>(p));
+    } else {
+      const uint2 w = *reinterpret_cast<const uint2*>(p);
+      const float2 a = unpack2<TYPE>(w.x), b = unpack2<TYPE>(w.y);
+      v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+    }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? load1<TYPE>(base, at + i) : 0.f;
+    for (int i = 0; i < W; ++i) v[i] = c + i < cols ? load1<TYPE>(p, i) : 0.f;
   }
 }
 
-template <int TYPE>
-__device__ __forceinline__ void store8(const float (&v)[8], void* base, size_t at, int c, int cols, bool vec) {
-  if (vec && c + 8 <= cols) {
-    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + at) = pack8<TYPE>(v);
+template <int TYPE, int W>
+__device__ __forceinline__ void storen(const float (&v)[W], void* base, size_t at, int c, int cols, bool vec) {
+  uint16_t* p = static_cast<uint16_t*>(base) + at;
+  if (vec && c + W <= cols) {
+    if constexpr (W == 8) *reinterpret_cast<uint4*>(p) = pack8<TYPE>(v);
+    else *reinterpret_cast<uint2*>(p) = make_uint2(pack2<TYPE>(v[0], v[1]), pack2<TYPE>(v[2], v[3]));
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (c + i < cols) store1<TYPE>(base, at + i, v[i]);
+    for (int i = 0; i < W; ++i)
+      if (c + i < cols) store1<TYPE>(p, i, v[i]);
   }
 }
 
@@ -113,24 +122,25 @@ __device__ __forceinline__ float act_fwd(float z) {
   return z;
 }
 
-// The same for eight values and an activation known at run time: one branch for all.
-__device__ __forceinline__ void act_fwd8(float (&v)[8], int act) {
+// The same for neighbours and an activation known at run time: one branch for all.
+template <int W>
+__device__ __forceinline__ void act_fwd_n(float (&v)[W], int act) {
   switch (act) {
     case kActRelu:
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = act_fwd<kActRelu>(v[i]);
+      for (int i = 0; i < W; ++i) v[i] = act_fwd<kActRelu>(v[i]);
       break;
     case kActGelu:
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = act_fwd<kActGelu>(v[i]);
+      for (int i = 0; i < W; ++i) v[i] = act_fwd<kActGelu>(v[i]);
       break;
     case kActGeluTanh:
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = act_fwd<kActGeluTanh>(v[i]);
+      for (int i = 0; i < W; ++i) v[i] = act_fwd<kActGeluTanh>(v[i]);
       break;
     case kActSilu:
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = act_fwd<kActSilu>(v[i]);
+      for (int i = 0; i < W; ++i) v[i] = act_fwd<kActSilu>(v[i]);
       break;
     default: break;
   }
@@ -204,6 +214,16 @@ __device__ __forceinline__ void drop8(float (&v)[8], const DropArgs& d, uint64_t
     v[2 * i] = (w[i] & 0xFFFFu) >= d.thr ? v[2 * i] * d.scale : 0.f;
     v[2 * i + 1] = (w[i] >> 16) >= d.thr ? v[2 * i + 1] * d.scale : 0.f;
   }
+}
+
+// The same for columns c .. c+3 (c a multiple of 4).
+__device__ __forceinline__ void drop4(float (&v)[4], const DropArgs& d, uint64_t off, int row, int c) {
+  const uint4 b = drop_bits(d, off, row, c >> 3);
+  const uint32_t lo = c & 4 ? b.z : b.x, hi = c & 4 ? b.w : b.y;
+  v[0] = (lo & 0xFFFFu) >= d.thr ? v[0] * d.scale : 0.f;
+  v[1] = (lo >> 16) >= d.thr ? v[1] * d.scale : 0.f;
+  v[2] = (hi & 0xFFFFu) >= d.thr ? v[2] * d.scale : 0.f;
+  v[3] = (hi >> 16) >= d.thr ? v[3] * d.scale : 0.f;
 }
 
 }  // namespace mlpg

@@ -21,15 +21,15 @@ __global__ void __launch_bounds__(256) dropout_kernel(DropoutArgs p, int groups,
   for (long i = blockIdx.x * 256L + threadIdx.x; i < total; i += gridDim.x * 256L) {
     const int r = (int)(i / groups), g = (int)(i % groups), c = 8 * g;
     float v[8];
-    load8<TYPE>(v, p.X, (size_t)r * p.ldx + c, c, p.M, vx);
+    loadn<TYPE, 8>(v, p.X, (size_t)r * p.ldx + c, c, p.M, vx);
     if (p.drop.thr) drop8(v, p.drop, off, r, g);
     if (p.res) {
       float q[8];
-      load8<TYPE>(q, p.res, (size_t)r * p.ldr + c, c, p.M, vr);
+      loadn<TYPE, 8>(q, p.res, (size_t)r * p.ldr + c, c, p.M, vr);
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] += q[j];
     }
-    store8<TYPE>(v, p.Y, (size_t)r * p.ldy + c, c, p.M, vy);
+    storen<TYPE, 8>(v, p.Y, (size_t)r * p.ldy + c, c, p.M, vy);
   }
 }
 
@@ -44,15 +44,15 @@ __global__ void __launch_bounds__(256) act_grad_kernel(ActGradArgs p, bool vy, b
   if (c < p.M)
     for (int r = rr; r < p.N; r += 32) {
       float v[8];
-      load8<TYPE>(v, p.dY, (size_t)r * p.lddy + c, c, p.M, vy);
+      loadn<TYPE, 8>(v, p.dY, (size_t)r * p.lddy + c, c, p.M, vy);
       if constexpr (ACT != kActNone) {
         float z[8];
-        load8<TYPE>(z, p.Z, (size_t)r * p.ldz + c, c, p.M, vz);
+        loadn<TYPE, 8>(z, p.Z, (size_t)r * p.ldz + c, c, p.M, vz);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] *= act_slope<ACT>(z[j]);
       }
       if (p.drop.thr) drop8(v, p.drop, off, r, g);
-      if (p.dZ) store8<TYPE>(v, p.dZ, (size_t)r * p.lddz + c, c, p.M, vd);
+      if (p.dZ) storen<TYPE, 8>(v, p.dZ, (size_t)r * p.lddz + c, c, p.M, vd);
 #pragma unroll
       for (int j = 0; j < 8; ++j) sum[j] += v[j];
     }

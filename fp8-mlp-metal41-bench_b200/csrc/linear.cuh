@@ -46,7 +46,7 @@ struct EpiArgs {
 template <int TYPE>
 __device__ __forceinline__ void add_bias8(float (&v)[8], const EpiArgs& p, int c) {
   float b[8];
-  load8<TYPE>(b, p.bias, (size_t)c, c, p.cols, p.bias_vec);
+  loadn<TYPE, 8>(b, p.bias, (size_t)c, c, p.cols, p.bias_vec);
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] += b[i];
 }

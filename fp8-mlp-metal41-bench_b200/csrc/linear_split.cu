@@ -159,51 +159,61 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<OP, BN>::PER_SM)
     while (global_ns() - t0 < 100000ull) {}
   }
   __syncwarp();
-  cluster_sync();
+  if (S > 1) cluster_sync();
+  else __syncthreads();
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem_base, C::TMEM_COLS);
   }
 
-  // this CTA's share of the tile's 8-column groups
+  // The tile's rows go round the cluster.  A thread finishes four columns: the 32 lanes
+  // then read 512 contiguous bytes of each partial sum, which is what the SM-to-SM
+  // network carries best (eight columns per thread, half of the lanes' 16-byte units at
+  // a time, took twice as long).
   const uint64_t off = drop_offset(p.drop);
-  const uint32_t mine = smem_u32(part);
-  for (int i = rank * kSplitThreads + (int)threadIdx.x; i < nrows * 16; i += S * kSplitThreads) {
-    const int n = i >> 4, row = r0 + n, c = c0 + 8 * (i & 15);
-    if (c >= p.cols) continue;
-    const uint32_t at = mine + (uint32_t)(n * 128 + 8 * (i & 15)) * 4u;
-    // every partial sum's load is in flight before the first is added
-    float4 x[kMaxSplit], y[kMaxSplit];
+  const int c = c0 + 4 * lane;
+  if (c < p.cols) {
+    for (int n = rank + S * warp; n < nrows; n += S * (kSplitThreads / 32)) {
+      const int row = r0 + n;
+      const uint32_t at = smem_u32(part) + (uint32_t)(n * 128 + 4 * lane) * 4u;
+      // every partial sum's load is in flight before the first is added
+      float4 x[kMaxSplit];
 #pragma unroll
-    for (int s = 0; s < kMaxSplit; ++s) {
-      if (s >= S) break;
-      uint32_t a;
-      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(at), "r"(s));
-      x[s] = ld_dsmem_f4(a);
-      y[s] = ld_dsmem_f4(a + 16u);
-    }
-    float v[8] = {};
+      for (int s = 0; s < kMaxSplit; ++s)
+        if (s < S) x[s] = ld_dsmem_f4(mapa_addr(at, (uint32_t)s));
+      float v[4] = {};
 #pragma unroll
-    for (int s = 0; s < kMaxSplit; ++s) {
-      if (s >= S) break;
-      v[0] += x[s].x; v[1] += x[s].y; v[2] += x[s].z; v[3] += x[s].w;
-      v[4] += y[s].x; v[5] += y[s].y; v[6] += y[s].z; v[7] += y[s].w;
-    }
-    if constexpr (OP == kOpLinear) {
-      if (p.bias) add_bias8<TYPE>(v, p, c);
-      if (p.pre) store8<TYPE>(v, p.pre, (size_t)row * p.ldz + c, c, p.cols, p.pre_vec);
-      act_fwd8(v, p.act);
-      if (p.drop.thr) drop8(v, p.drop, off, row, c >> 3);
-    }
-    if (p.res) {
-      float r[8];
-      load8<TYPE>(r, p.res, (size_t)row * p.ldr + c, c, p.cols, p.res_vec);
+      for (int s = 0; s < kMaxSplit; ++s)
+        if (s < S) {
+          v[0] += x[s].x;
+          v[1] += x[s].y;
+          v[2] += x[s].z;
+          v[3] += x[s].w;
+        }
+      if constexpr (OP == kOpLinear) {
+        float b[4];
+        if (p.bias) {
+          loadn<TYPE, 4>(b, p.bias, (size_t)c, c, p.cols, p.bias_vec);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] += r[j];
+          for (int j = 0; j < 4; ++j) v[j] += b[j];
+        }
+        if (p.pre) storen<TYPE, 4>(v, p.pre, (size_t)row * p.ldz + c, c, p.cols, p.pre_vec);
+        act_fwd_n(v, p.act);
+        if (p.drop.thr) drop4(v, p.drop, off, row, c);
+      }
+      if (p.res) {
+        float r[4];
+        loadn<TYPE, 4>(r, p.res, (size_t)row * p.ldr + c, c, p.cols, p.res_vec);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] += r[j];
+      }
+      storen<TYPE, 4>(v, p.out, (size_t)row * p.ldo + c, c, p.cols, p.out_vec);
     }
-    store8<TYPE>(v, p.out, (size_t)row * p.ldo + c, c, p.cols, p.out_vec);
   }
-  cluster_sync();   // no CTA leaves while another reads its partial sums
+  // no CTA leaves while another reads its partial sums; nothing is handed over, so the
+  // barrier need not wait for the stores above
+  __syncwarp();
+  if (S > 1) cluster_sync_relaxed();
 }
 
 template <int OP, int TYPE, int BN>
