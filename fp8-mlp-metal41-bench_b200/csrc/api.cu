@@ -725,9 +725,14 @@ int make_dropout(const gemm_dropout_args* in, DropArgs* out) {
   if (!(in->p >= 0.0 && in->p <= 1.0)) return fail(GEMM_ERR_ARGS, "dropout probability %g not in 0..1", in->p);
   if (reinterpret_cast<uintptr_t>(in->offset_ptr) & 7u)
     return fail(GEMM_ERR_ARGS, "offset_ptr is not 8-byte aligned");
-  out->thr = (uint32_t)std::nearbyint(in->p * 65536.0);
-  out->scale = out->thr < 65536u ? 65536.f / (float)(65536u - out->thr) : 0.f;
-  out->seed = in->seed;
+  const uint32_t t = (uint32_t)std::nearbyint(in->p * 65536.0);
+  out->on = t > 0;
+  out->last = (uint32_t)(((uint64_t)t << 16) - 1);
+  out->scale = t < 65536u ? 65536.f / (float)(65536u - t) : 0.f;
+  for (uint32_t r = 0; r < 10; ++r) {
+    out->key[r][0] = (uint32_t)in->seed + r * 0x9E3779B9u;
+    out->key[r][1] = (uint32_t)(in->seed >> 32) + r * 0xBB67AE85u;
+  }
   out->offset = in->offset;
   out->offset_ptr = in->offset_ptr;
   return GEMM_OK;

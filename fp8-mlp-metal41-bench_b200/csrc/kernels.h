@@ -90,9 +90,11 @@ enum LayerAct : int { kActNone = 0, kActRelu = 1, kActGelu = 2, kActGeluTanh = 3
 enum LinearOp : int { kOpLinear = 0, kOpDx = 1, kOpDw = 2 };          // GEMM_OP_*
 
 struct DropArgs {
-  uint32_t thr = 0;     // an element is dropped where its 16-bit number is below; 0: no dropout
-  float scale = 1.f;    // 65536 / (65536 - thr); 0 where everything is dropped
-  uint64_t seed = 0, offset = 0;
+  int on = 0;
+  uint32_t last = 0;    // t 2^16 - 1: an element is dropped where its 16-bit number is below t
+  float scale = 1.f;    // 65536 / (65536 - t); 0 where everything is dropped
+  uint32_t key[10][2] = {};               // Philox's round keys
+  uint64_t offset = 0;
   const uint64_t* offset_ptr = nullptr;   // device: added to offset
 };
 

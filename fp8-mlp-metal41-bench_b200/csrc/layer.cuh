@@ -95,19 +95,43 @@ __device__ __forceinline__ void storen(const float (&v)[W], void* base, size_t a
 // ---- activations ------------------------------------------------------------------
 // gelu_tanh is written as z * sigmoid(2u), u = sqrt(2/pi) (z + 0.044715 z^3), which
 // equals 0.5 z (1 + tanh u) without the cancellation at large negative z.
-__device__ __forceinline__ float sigmoidf_(float t) { return __fdividef(1.f, 1.f + __expf(-t)); }
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ float ex2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// z between -m and m; NaN stays NaN
+__device__ __forceinline__ float clampf(float z, float m) {
+  float y;
+  asm("{\n\t.reg .f32 t;\n\tmin.NaN.f32 t, %1, %2;\n\tmax.NaN.f32 %0, t, %3;\n\t}" : "=f"(y) : "f"(z), "f"(m), "f"(-m));
+  return y;
+}
+
+// 1 / (1 + exp(-t))
+__device__ __forceinline__ float sigmoidf_(float t) { return rcp_approx(1.f + ex2_approx(-1.4426950408889634f * t)); }
 
 __device__ __forceinline__ float gelu_u2(float z) { return 1.5957691216057308f * (z + 0.044715f * z * z * z); }
 
-// Phi(z), the normal distribution, and e = exp(-z^2/2) by Abramowitz and Stegun 7.1.26:
-// erfc(x) = (a1 t + ... + a5 t^5) exp(-x^2), t = 1 / (1 + 0.3275911 x), off by at most
-// 1.5e-7: far below a 16-bit result's rounding, no branch, and the slope reuses e.
-__device__ __forceinline__ float normal_cdf(float z, float& e) {
-  const float t = __fdividef(1.f, 1.f + 0.23164189f * fabsf(z));   // 0.3275911 / sqrt(2)
-  e = __expf(-0.5f * z * z);
-  const float poly = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
-  const float tail = 0.5f * poly * e;
-  return z < 0.f ? tail : 1.f - tail;
+// e = exp(-a^2/2) and Phi(-a), the normal distribution's tail, for a >= 0 by Abramowitz
+// and Stegun 7.1.26: erfc(x) = (a1 t + ... + a5 t^5) exp(-x^2), t = 1 / (1 + 0.3275911 x),
+// off by at most 1.5e-7: far below a 16-bit result's rounding, no branch, and the slope
+// reuses e.  The coefficients here are halved (Phi(-a) = erfc(x) / 2), x = a / sqrt(2);
+// the tail comes without its factor e.
+__device__ __forceinline__ float normal_tail(float a, float& e) {
+  const float t = rcp_approx(fmaf(0.23164189f, a, 1.f));
+  e = ex2_approx(-0.72134752044448170f * a * a);
+  float q = fmaf(t, 0.5307027145f, -0.7265760135f);
+  q = fmaf(t, q, 0.7107068705f);
+  q = fmaf(t, q, -0.142248368f);
+  q = fmaf(t, q, 0.127414796f);
+  return q * t;
 }
 
 template <int ACT>
@@ -115,7 +139,8 @@ __device__ __forceinline__ float act_fwd(float z) {
   if constexpr (ACT == kActRelu) return z < 0.f ? 0.f : z;   // NaN stays NaN
   if constexpr (ACT == kActGelu) {
     float e;
-    return z * normal_cdf(z, e);
+    const float tail = normal_tail(fabsf(z), e) * e;
+    return z * (z < 0.f ? tail : 1.f - tail);
   }
   if constexpr (ACT == kActGeluTanh) return z * sigmoidf_(gelu_u2(z));
   if constexpr (ACT == kActSilu) return z * sigmoidf_(z);
@@ -153,18 +178,20 @@ template <int ACT>
 __device__ __forceinline__ float act_slope(float z) {
   if constexpr (ACT == kActRelu) return z > 0.f ? 1.f : (z <= 0.f ? 0.f : z);
   if constexpr (ACT == kActGelu) {
-    z = z > 30.f ? 30.f : (z < -30.f ? -30.f : z);
-    float e;
-    const float phi = normal_cdf(z, e);
-    return phi + z * e * 0.3989422804014327f;
+    // slope(-a) = 1 - slope(a)
+    float a, e;
+    asm("min.NaN.f32 %0, %1, 0f41F00000;" : "=f"(a) : "f"(fabsf(z)));   // 30
+    const float tail = normal_tail(a, e);
+    const float h = e * fmaf(0.3989422804014327f, a, -tail);
+    return z < 0.f ? -h : 1.f + h;
   }
   if constexpr (ACT == kActGeluTanh) {
-    z = z > 30.f ? 30.f : (z < -30.f ? -30.f : z);
+    z = clampf(z, 30.f);
     const float q = sigmoidf_(gelu_u2(z));
     return q + z * q * (1.f - q) * (1.5957691216057308f * (1.f + 0.134145f * z * z));
   }
   if constexpr (ACT == kActSilu) {
-    z = z > 80.f ? 80.f : (z < -80.f ? -80.f : z);
+    z = clampf(z, 80.f);
     const float q = sigmoidf_(z);
     return q * (1.f + z * (1.f - q));
   }
@@ -176,54 +203,46 @@ __device__ __forceinline__ float act_slope(float z) {
 // as 1, 2, 3", SC 2011).  The counter is (column / 8, row, offset), the key the
 // seed, so any tile shape computes the same mask; eight neighbours of a row share
 // one evaluation, 16 bits each, low half-words first.  16 bits per element halve the
-// integer work that would otherwise bound the elementwise kernels (about 80
-// instructions per evaluation); p is rounded to a multiple of 2^-16 and the scale is
-// that of the rounded p, so the expectation is exact.
-__device__ __forceinline__ uint4 philox4x32_10(uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3, uint32_t k0,
-                                               uint32_t k1) {
+// integer work, which shows in the elementwise kernels; p is rounded to a multiple of
+// 2^-16 and the scale is that of the rounded p, so the expectation is exact.  The ten
+// round keys come ready-made in the kernel's arguments.
+__device__ __forceinline__ uint4 drop_bits(const DropArgs& d, uint64_t off, int row, int g) {
+  uint32_t c0 = (uint32_t)g, c1 = (uint32_t)row, c2 = (uint32_t)off, c3 = (uint32_t)(off >> 32);
 #pragma unroll
   for (int r = 0; r < 10; ++r) {
     const uint64_t p0 = (uint64_t)0xD2511F53u * c0, p1 = (uint64_t)0xCD9E8D57u * c2;
-    const uint32_t n0 = (uint32_t)(p1 >> 32) ^ c1 ^ k0, n2 = (uint32_t)(p0 >> 32) ^ c3 ^ k1;
+    c0 = (uint32_t)(p1 >> 32) ^ c1 ^ d.key[r][0];
+    c2 = (uint32_t)(p0 >> 32) ^ c3 ^ d.key[r][1];
     c1 = (uint32_t)p1;
     c3 = (uint32_t)p0;
-    c0 = n0;
-    c2 = n2;
-    k0 += 0x9E3779B9u;
-    k1 += 0xBB67AE85u;
   }
   return make_uint4(c0, c1, c2, c3);
 }
 
 __device__ __forceinline__ uint64_t drop_offset(const DropArgs& d) {
-  return d.offset + ((d.thr && d.offset_ptr) ? *d.offset_ptr : 0ull);
+  return d.offset + ((d.on && d.offset_ptr) ? *d.offset_ptr : 0ull);
 }
 
-// The eight 16-bit numbers of columns 8 g .. 8 g + 7 of `row`.
-__device__ __forceinline__ uint4 drop_bits(const DropArgs& d, uint64_t off, int row, int g) {
-  return philox4x32_10((uint32_t)g, (uint32_t)row, (uint32_t)off, (uint32_t)(off >> 32), (uint32_t)d.seed,
-                       (uint32_t)(d.seed >> 32));
+// Two neighbours and their word of 16-bit numbers u.  u < t is u * 2^16 <= t * 2^16 - 1
+// = d.last, which the upper half-word's compare needs no shift for.  A dropped element is
+// 0 whatever it held, infinities and NaN included.
+__device__ __forceinline__ void drop2(float& lo, float& hi, const DropArgs& d, uint32_t w) {
+  lo = (w << 16) <= d.last ? 0.f : lo * d.scale;
+  hi = w <= d.last ? 0.f : hi * d.scale;
 }
 
-// A dropped element is 0 whatever it held, infinities and NaN included.
-__device__ __forceinline__ void drop8(float (&v)[8], const DropArgs& d, uint64_t off, int row, int g) {
-  const uint4 b = drop_bits(d, off, row, g);
-  const uint32_t w[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[2 * i] = (w[i] & 0xFFFFu) >= d.thr ? v[2 * i] * d.scale : 0.f;
-    v[2 * i + 1] = (w[i] >> 16) >= d.thr ? v[2 * i + 1] * d.scale : 0.f;
-  }
+__device__ __forceinline__ void drop8(float (&v)[8], const DropArgs& d, uint4 b) {
+  drop2(v[0], v[1], d, b.x);
+  drop2(v[2], v[3], d, b.y);
+  drop2(v[4], v[5], d, b.z);
+  drop2(v[6], v[7], d, b.w);
 }
 
-// The same for columns c .. c+3 (c a multiple of 4).
+// Columns c .. c+3 (c a multiple of 4).
 __device__ __forceinline__ void drop4(float (&v)[4], const DropArgs& d, uint64_t off, int row, int c) {
   const uint4 b = drop_bits(d, off, row, c >> 3);
-  const uint32_t lo = c & 4 ? b.z : b.x, hi = c & 4 ? b.w : b.y;
-  v[0] = (lo & 0xFFFFu) >= d.thr ? v[0] * d.scale : 0.f;
-  v[1] = (lo >> 16) >= d.thr ? v[1] * d.scale : 0.f;
-  v[2] = (hi & 0xFFFFu) >= d.thr ? v[2] * d.scale : 0.f;
-  v[3] = (hi >> 16) >= d.thr ? v[3] * d.scale : 0.f;
+  drop2(v[0], v[1], d, c & 4 ? b.z : b.x);
+  drop2(v[2], v[3], d, c & 4 ? b.w : b.y);
 }
 
 }  // namespace mlpg

@@ -364,9 +364,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
               }
 #pragma unroll
               for (int i = 0; i < 16; ++i) v[i >> 3][i & 7] = act_fwd<ACT>(v[i >> 3][i & 7]);
-              if (p.e.drop.thr) {
-                drop8(v[0], p.e.drop, off, row, c >> 3);
-                drop8(v[1], p.e.drop, off, row, (c >> 3) + 1);
+              if (p.e.drop.on) {
+                drop8(v[0], p.e.drop, drop_bits(p.e.drop, off, row, c >> 3));
+                drop8(v[1], p.e.drop, drop_bits(p.e.drop, off, row, (c >> 3) + 1));
               }
             }
             uint4 *at0 = unit(sb, lane, j), *at1 = unit(sb, lane, j + 1);

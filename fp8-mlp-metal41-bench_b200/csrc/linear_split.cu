@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<OP, BN>::PER_SM)
         }
         if (p.pre) storen<TYPE, 4>(v, p.pre, (size_t)row * p.ldz + c, c, p.cols, p.pre_vec);
         act_fwd_n(v, p.act);
-        if (p.drop.thr) drop4(v, p.drop, off, row, c);
+        if (p.drop.on) drop4(v, p.drop, off, row, c);
       }
       if (p.res) {
         float r[4];
