@@ -92,110 +92,172 @@ __device__ __forceinline__ void storen(const float (&v)[W], void* base, size_t a
   }
 }
 
+// ---- pairs of f32 -------------------------------------------------------------------
+// sm_100 multiplies, adds and fuses two f32 per instruction; the epilogues are bound by
+// instructions issued, so their arithmetic goes in pairs.
+struct f32x2 {
+  unsigned long long v;
+};
+__device__ __forceinline__ f32x2 pair2(float lo, float hi) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ f32x2 pair2(float x) { return pair2(x, x); }
+__device__ __forceinline__ void split2(f32x2 a, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(a.v));
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+template <typename F>
+__device__ __forceinline__ f32x2 each2(f32x2 a, F f) {
+  float lo, hi;
+  split2(a, lo, hi);
+  return pair2(f(lo), f(hi));
+}
+
 // ---- activations ------------------------------------------------------------------
-// gelu_tanh is written as z * sigmoid(2u), u = sqrt(2/pi) (z + 0.044715 z^3), which
-// equals 0.5 z (1 + tanh u) without the cancellation at large negative z.
-__device__ __forceinline__ float rcp_approx(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
+__device__ __forceinline__ f32x2 rcp2(f32x2 a) {
+  return each2(a, [](float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+  });
+}
+__device__ __forceinline__ f32x2 ex2_2(f32x2 a) {   // 2^a
+  return each2(a, [](float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+  });
+}
+__device__ __forceinline__ f32x2 abs2(f32x2 a) {
+  return each2(a, [](float x) { return fabsf(x); });
+}
+// between -m and m; NaN stays NaN
+__device__ __forceinline__ f32x2 clamp2(f32x2 a, float m) {
+  return each2(a, [m](float x) {
+    float y;
+    asm("{\n\t.reg .f32 t;\n\tmin.NaN.f32 t, %1, %2;\n\tmax.NaN.f32 %0, t, %3;\n\t}"
+        : "=f"(y)
+        : "f"(x), "f"(m), "f"(-m));
+    return y;
+  });
 }
 
-__device__ __forceinline__ float ex2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
+// 1 / (1 + 2^x): the sigmoid of -x / log2(e)
+__device__ __forceinline__ f32x2 sigmoid2(f32x2 x) { return rcp2(add2(ex2_2(x), pair2(1.f))); }
+
+// gelu_tanh is z * sigmoid(2u), u = sqrt(2/pi) (z + 0.044715 z^3), which equals
+// 0.5 z (1 + tanh u) without the cancellation at large negative z; -2u log2(e) here.
+__device__ __forceinline__ f32x2 gelu_2u(f32x2 z) {
+  return mul2(z, fma2(mul2(z, z), pair2(-0.10294324f), pair2(-2.3022082f)));
 }
 
-// z between -m and m; NaN stays NaN
-__device__ __forceinline__ float clampf(float z, float m) {
-  float y;
-  asm("{\n\t.reg .f32 t;\n\tmin.NaN.f32 t, %1, %2;\n\tmax.NaN.f32 %0, t, %3;\n\t}" : "=f"(y) : "f"(z), "f"(m), "f"(-m));
-  return y;
-}
-
-// 1 / (1 + exp(-t))
-__device__ __forceinline__ float sigmoidf_(float t) { return rcp_approx(1.f + ex2_approx(-1.4426950408889634f * t)); }
-
-__device__ __forceinline__ float gelu_u2(float z) { return 1.5957691216057308f * (z + 0.044715f * z * z * z); }
-
-// e = exp(-a^2/2) and Phi(-a), the normal distribution's tail, for a >= 0 by Abramowitz
+// e = exp(-a^2/2) and -Phi(-a), the normal distribution's tail, for a >= 0 by Abramowitz
 // and Stegun 7.1.26: erfc(x) = (a1 t + ... + a5 t^5) exp(-x^2), t = 1 / (1 + 0.3275911 x),
 // off by at most 1.5e-7: far below a 16-bit result's rounding, no branch, and the slope
-// reuses e.  The coefficients here are halved (Phi(-a) = erfc(x) / 2), x = a / sqrt(2);
-// the tail comes without its factor e.
-__device__ __forceinline__ float normal_tail(float a, float& e) {
-  const float t = rcp_approx(fmaf(0.23164189f, a, 1.f));
-  e = ex2_approx(-0.72134752044448170f * a * a);
-  float q = fmaf(t, 0.5307027145f, -0.7265760135f);
-  q = fmaf(t, q, 0.7107068705f);
-  q = fmaf(t, q, -0.142248368f);
-  q = fmaf(t, q, 0.127414796f);
-  return q * t;
+// reuses e.  The coefficients here are halved and negated (Phi(-a) = erfc(x) / 2),
+// x = a / sqrt(2); the tail comes without its factor e.
+__device__ __forceinline__ f32x2 normal_tail2(f32x2 a, f32x2& e) {
+  const f32x2 t = rcp2(fma2(pair2(0.23164189f), a, pair2(1.f)));
+  e = ex2_2(mul2(mul2(a, a), pair2(-0.72134752044448170f)));
+  f32x2 q = fma2(t, pair2(-0.5307027145f), pair2(0.7265760135f));
+  q = fma2(t, q, pair2(-0.7107068705f));
+  q = fma2(t, q, pair2(0.142248368f));
+  q = fma2(t, q, pair2(-0.127414796f));
+  return mul2(q, t);
+}
+
+// z < 0 ? neg : pos, element by element (NaN takes pos)
+__device__ __forceinline__ f32x2 by_sign2(f32x2 z, f32x2 neg, f32x2 pos) {
+  float zl, zh, nl, nh, pl, ph;
+  split2(z, zl, zh);
+  split2(neg, nl, nh);
+  split2(pos, pl, ph);
+  return pair2(zl < 0.f ? nl : pl, zh < 0.f ? nh : ph);
 }
 
 template <int ACT>
-__device__ __forceinline__ float act_fwd(float z) {
-  if constexpr (ACT == kActRelu) return z < 0.f ? 0.f : z;   // NaN stays NaN
+__device__ __forceinline__ f32x2 act_fwd2(f32x2 z) {
+  if constexpr (ACT == kActRelu) return by_sign2(z, pair2(0.f), z);   // NaN stays NaN
   if constexpr (ACT == kActGelu) {
-    float e;
-    const float tail = normal_tail(fabsf(z), e) * e;
-    return z * (z < 0.f ? tail : 1.f - tail);
+    f32x2 e;
+    const f32x2 tail = normal_tail2(abs2(z), e), p = mul2(tail, e);
+    return mul2(z, by_sign2(z, mul2(p, pair2(-1.f)), add2(p, pair2(1.f))));
   }
-  if constexpr (ACT == kActGeluTanh) return z * sigmoidf_(gelu_u2(z));
-  if constexpr (ACT == kActSilu) return z * sigmoidf_(z);
+  if constexpr (ACT == kActGeluTanh) return mul2(z, sigmoid2(gelu_2u(z)));
+  if constexpr (ACT == kActSilu) return mul2(z, sigmoid2(mul2(z, pair2(-1.4426950408889634f))));
   return z;
 }
 
-// The same for neighbours and an activation known at run time: one branch for all.
+template <int ACT, int W>
+__device__ __forceinline__ void act_fwd_n(float (&v)[W]) {
+#pragma unroll
+  for (int i = 0; i < W; i += 2) split2(act_fwd2<ACT>(pair2(v[i], v[i + 1])), v[i], v[i + 1]);
+}
+
+// The same for an activation known at run time: one branch for all.
 template <int W>
 __device__ __forceinline__ void act_fwd_n(float (&v)[W], int act) {
   switch (act) {
-    case kActRelu:
-#pragma unroll
-      for (int i = 0; i < W; ++i) v[i] = act_fwd<kActRelu>(v[i]);
-      break;
-    case kActGelu:
-#pragma unroll
-      for (int i = 0; i < W; ++i) v[i] = act_fwd<kActGelu>(v[i]);
-      break;
-    case kActGeluTanh:
-#pragma unroll
-      for (int i = 0; i < W; ++i) v[i] = act_fwd<kActGeluTanh>(v[i]);
-      break;
-    case kActSilu:
-#pragma unroll
-      for (int i = 0; i < W; ++i) v[i] = act_fwd<kActSilu>(v[i]);
-      break;
+    case kActRelu: act_fwd_n<kActRelu, W>(v); break;
+    case kActGelu: act_fwd_n<kActGelu, W>(v); break;
+    case kActGeluTanh: act_fwd_n<kActGeluTanh, W>(v); break;
+    case kActSilu: act_fwd_n<kActSilu, W>(v); break;
     default: break;
   }
 }
 
 // act'(z).  z is a stored pre-activation, which f16 may have rounded to an
 // infinity: beyond the clamps every slope is 0 or 1 to f32 precision, so an
-// infinite z gets its limit instead of inf * 0.  NaN passes the comparisons.
+// infinite z gets its limit instead of inf * 0.  NaN stays NaN.
 template <int ACT>
-__device__ __forceinline__ float act_slope(float z) {
-  if constexpr (ACT == kActRelu) return z > 0.f ? 1.f : (z <= 0.f ? 0.f : z);
+__device__ __forceinline__ f32x2 act_slope2(f32x2 z) {
+  const f32x2 one = pair2(1.f), minus = pair2(-1.f);
+  if constexpr (ACT == kActRelu) return each2(z, [](float x) { return x > 0.f ? 1.f : (x <= 0.f ? 0.f : x); });
   if constexpr (ACT == kActGelu) {
     // slope(-a) = 1 - slope(a)
-    float a, e;
-    asm("min.NaN.f32 %0, %1, 0f41F00000;" : "=f"(a) : "f"(fabsf(z)));   // 30
-    const float tail = normal_tail(a, e);
-    const float h = e * fmaf(0.3989422804014327f, a, -tail);
-    return z < 0.f ? -h : 1.f + h;
+    f32x2 e;
+    const f32x2 a = each2(z, [](float x) {
+      float y;
+      asm("min.NaN.f32 %0, %1, 0f41F00000;" : "=f"(y) : "f"(fabsf(x)));   // 30
+      return y;
+    });
+    const f32x2 tail = normal_tail2(a, e);
+    const f32x2 h = fma2(e, fma2(a, pair2(0.3989422804014327f), tail), pair2(0.5f));
+    // 0.5 +- (0.5 + h), the sign z's; 0.5 + h >= 0
+    float zl, zh, hl, hh;
+    split2(z, zl, zh);
+    split2(h, hl, hh);
+    return add2(pair2(copysignf(hl, zl), copysignf(hh, zh)), pair2(0.5f));
   }
   if constexpr (ACT == kActGeluTanh) {
-    z = clampf(z, 30.f);
-    const float q = sigmoidf_(gelu_u2(z));
-    return q + z * q * (1.f - q) * (1.5957691216057308f * (1.f + 0.134145f * z * z));
+    // q + z q (1 - q) (2u)'
+    z = clamp2(z, 30.f);
+    const f32x2 q = sigmoid2(gelu_2u(z));
+    const f32x2 d = mul2(z, fma2(mul2(z, z), pair2(0.21406445f), pair2(1.5957691216057308f)));
+    return mul2(q, fma2(d, fma2(q, minus, one), one));
   }
   if constexpr (ACT == kActSilu) {
-    z = clampf(z, 80.f);
-    const float q = sigmoidf_(z);
-    return q * (1.f + z * (1.f - q));
+    z = clamp2(z, 80.f);
+    const f32x2 q = sigmoid2(mul2(z, pair2(-1.4426950408889634f)));
+    return mul2(q, fma2(z, fma2(q, minus, one), one));
   }
-  return 1.f;
+  return one;
 }
 
 // ---- dropout ------------------------------------------------------------------------
@@ -227,8 +289,10 @@ __device__ __forceinline__ uint64_t drop_offset(const DropArgs& d) {
 // = d.last, which the upper half-word's compare needs no shift for.  A dropped element is
 // 0 whatever it held, infinities and NaN included.
 __device__ __forceinline__ void drop2(float& lo, float& hi, const DropArgs& d, uint32_t w) {
-  lo = (w << 16) <= d.last ? 0.f : lo * d.scale;
-  hi = w <= d.last ? 0.f : hi * d.scale;
+  float a, b;
+  split2(mul2(pair2(lo, hi), pair2(d.scale)), a, b);
+  lo = (w << 16) <= d.last ? 0.f : a;
+  hi = w <= d.last ? 0.f : b;
 }
 
 __device__ __forceinline__ void drop8(float (&v)[8], const DropArgs& d, uint4 b) {

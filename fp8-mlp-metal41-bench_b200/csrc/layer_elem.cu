@@ -9,6 +9,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "layer.cuh"
 #include "ptx.cuh"
@@ -24,60 +25,100 @@ bool vec_rows(const void* p, long ld) { return (reinterpret_cast<uintptr_t>(p) &
 
 constexpr int kDepth = 4;
 
-// Eight elements from global to shared memory: cp.async where the rows allow it, else
-// (and past the row's end, where zeros go) plain loads.  Read once: no L1.
-__device__ __forceinline__ void fetch8(uint4* dst, const void* base, size_t at, int c, int cols, bool vec) {
-  const uint16_t* p = static_cast<const uint16_t*>(base) + at;
-  if (vec && c + 8 <= cols) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(p) : "memory");
+// A thread's walk down its rows of one operand: the next row's address, and whether its
+// eight columns are one aligned 16-byte unit.
+struct Walk {
+  const uint16_t* p;
+  long step;      // elements from one of the thread's rows to the next
+  bool unit;
+};
+
+__device__ __forceinline__ Walk walk(const void* base, long ld, bool vec, int r, int rows, int c, int cols) {
+  return Walk{static_cast<const uint16_t*>(base) + (size_t)r * ld + c, ld * rows, vec && c + 8 <= cols};
+}
+
+// The walk's row to shared memory: cp.async where it is one unit, else plain loads, with
+// zeros past the row's end.  Every element is read once: L1 is passed by.
+__device__ __forceinline__ void fetch8(uint32_t dst, Walk& w, int c, int cols) {
+  if (w.unit) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(w.p) : "memory");
   } else {
-    uint32_t w[4];
+    uint32_t q[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      w[i] = (c + 2 * i < cols ? p[2 * i] : 0u) | ((uint32_t)(c + 2 * i + 1 < cols ? p[2 * i + 1] : 0u) << 16);
-    *dst = make_uint4(w[0], w[1], w[2], w[3]);
+      q[i] = (c + 2 * i < cols ? w.p[2 * i] : 0u) | ((uint32_t)(c + 2 * i + 1 < cols ? w.p[2 * i + 1] : 0u) << 16);
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(q[0]), "r"(q[1]), "r"(q[2]), "r"(q[3])
+                 : "memory");
   }
+  w.p += w.step;
 }
 __device__ __forceinline__ void fetch_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // all but the kDepth - 1 newest groups have landed
 __device__ __forceinline__ void fetch_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory"); }
 
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+template <int TYPE>
+__device__ __forceinline__ void put8(const float (&v)[8], Walk& w, int c, int cols) {
+  storen<TYPE, 8>(v, const_cast<uint16_t*>(w.p), 0, c, cols, w.unit);
+  w.p += w.step;
+}
+
+// One or two operands' rows pass through f(row, words of the first, of the second) in
+// order, from `r` on in steps of `rows`; `ring` is the thread's 16 bytes of slot 0.
+template <int OPS, typename F>
+__device__ __forceinline__ void stream_rows(uint32_t ring, Walk a, Walk b, int r, int rows, int n, int c, int cols, F f) {
+  constexpr uint32_t kOp = kThreads * 16, kSlot = OPS * kOp, kRing = kDepth * kSlot;
+  static_assert((kRing & (kRing - 1)) == 0, "power of two");
+  int next = r;
+  uint32_t in = 0, out = 0;
+  auto fetch = [&] {
+    if (next < n) {
+      fetch8(ring + in, a, c, cols);
+      if constexpr (OPS == 2) fetch8(ring + in + kOp, b, c, cols);
+    }
+    fetch_commit();
+    next += rows;
+    in = (in + kSlot) & (kRing - 1);
+  };
+#pragma unroll
+  for (int d = 0; d < kDepth - 1; ++d) fetch();
+  for (; r < n; r += rows) {
+    fetch();
+    f(r, [&] { fetch_wait(); return lds16(ring + out); }, [&] { return lds16(ring + out + kOp); });
+    out = (out + kSlot) & (kRing - 1);
+  }
+}
+
 template <int TYPE, bool RES>
 __global__ void __launch_bounds__(kThreads) dropout_kernel(const __grid_constant__ DropoutArgs p, int lx, bool vx, bool vr,
                                                            bool vy) {
-  __shared__ uint4 ring[kDepth][RES ? 2 : 1][kThreads];
+  __shared__ uint4 ring[kDepth * (RES ? 2 : 1) * kThreads];
   const int t = (int)threadIdx.x;
   const int g = (int)(blockIdx.x << lx) + (t & ((1 << lx) - 1)), c = 8 * g;
   if (c >= p.M) return;
   const uint64_t off = drop_offset(p.drop);
-  const long step = (long)gridDim.y * (kThreads >> lx);
-  long next = (long)blockIdx.y * (kThreads >> lx) + (t >> lx);
-  auto fetch = [&](int slot) {
-    if (next < p.N) {
-      fetch8(&ring[slot][0][t], p.X, (size_t)next * p.ldx + c, c, p.M, vx);
-      if constexpr (RES) fetch8(&ring[slot][1][t], p.res, (size_t)next * p.ldr + c, c, p.M, vr);
-    }
-    fetch_commit();
-    next += step;
-  };
-  long r = next;
-#pragma unroll
-  for (int d = 0; d < kDepth - 1; ++d) fetch(d);
-  for (int slot = 0; r < p.N; r += step, slot = (slot + 1) % kDepth) {
-    fetch((slot + kDepth - 1) % kDepth);
-    const uint4 b = p.drop.on ? drop_bits(p.drop, off, (int)r, g) : make_uint4(0, 0, 0, 0);
-    fetch_wait();
+  const int rows = (int)gridDim.y * (kThreads >> lx), r = (int)blockIdx.y * (kThreads >> lx) + (t >> lx);
+  Walk y = walk(p.Y, p.ldy, vy, r, rows, c, p.M);
+  stream_rows<RES ? 2 : 1>(smem_u32(ring + t), walk(p.X, p.ldx, vx, r, rows, c, p.M),
+                           walk(p.res, p.ldr, vr, r, rows, c, p.M), r, rows, p.N, c, p.M,
+                           [&](int row, auto first, auto second) {
+    const uint4 b = p.drop.on ? drop_bits(p.drop, off, row, g) : make_uint4(0, 0, 0, 0);
     float v[8];
-    unpack8<TYPE>(v, ring[slot][0][t]);
+    unpack8<TYPE>(v, first());
     if (p.drop.on) drop8(v, p.drop, b);
     if constexpr (RES) {
       float w[8];
-      unpack8<TYPE>(w, ring[slot][1][t]);
+      unpack8<TYPE>(w, second());
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] += w[j];
+      for (int j = 0; j < 8; j += 2) split2(add2(pair2(v[j], v[j + 1]), pair2(w[j], w[j + 1])), v[j], v[j + 1]);
     }
-    storen<TYPE, 8>(v, p.Y, (size_t)r * p.ldy + c, c, p.M, vy);
-  }
+    put8<TYPE>(v, y, c, p.M);
+  });
 }
 
 // A cluster's CTAs share the rows of one slab of columns.  Each thread's eight column
@@ -86,7 +127,7 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(const __grid_constant
 template <int TYPE, int ACT>
 __global__ void __launch_bounds__(kThreads, 4) act_grad_kernel(const __grid_constant__ ActGradArgs p, int lx, bool vy, bool vz,
                                                                bool vd) {
-  __shared__ uint4 ring[kDepth][ACT == kActNone ? 1 : 2][kThreads];
+  __shared__ uint4 ring[kDepth * (ACT == kActNone ? 1 : 2) * kThreads];
   float* part = reinterpret_cast<float*>(ring);   // the sums, once the ring is drained
   const int t = (int)threadIdx.x, ty = kThreads >> lx, tx = 1 << lx;
   const int S = (int)gridDim.y, rank = (int)blockIdx.y;   // the cluster is the grid's y
@@ -94,36 +135,27 @@ __global__ void __launch_bounds__(kThreads, 4) act_grad_kernel(const __grid_cons
   float sum[8] = {};
   if (c < p.M) {
     const uint64_t off = drop_offset(p.drop);
-    const long step = (long)S * ty;
-    long next = (long)rank * ty + (t >> lx);
-    auto fetch = [&](int slot) {
-      if (next < p.N) {
-        fetch8(&ring[slot][0][t], p.dY, (size_t)next * p.lddy + c, c, p.M, vy);
-        if constexpr (ACT != kActNone) fetch8(&ring[slot][1][t], p.Z, (size_t)next * p.ldz + c, c, p.M, vz);
-      }
-      fetch_commit();
-      next += step;
-    };
-    long r = next;
-#pragma unroll
-    for (int d = 0; d < kDepth - 1; ++d) fetch(d);
-    for (int slot = 0; r < p.N; r += step, slot = (slot + 1) % kDepth) {
-      fetch((slot + kDepth - 1) % kDepth);
-      const uint4 b = p.drop.on ? drop_bits(p.drop, off, (int)r, g) : make_uint4(0, 0, 0, 0);
-      fetch_wait();
+    const int rows = S * ty, r = rank * ty + (t >> lx);
+    Walk d = walk(p.dZ, p.lddz, vd, r, rows, c, p.M);
+    stream_rows<ACT == kActNone ? 1 : 2>(smem_u32(ring + t), walk(p.dY, p.lddy, vy, r, rows, c, p.M),
+                                         walk(p.Z, p.ldz, vz, r, rows, c, p.M), r, rows, p.N, c, p.M,
+                                         [&](int row, auto first, auto second) {
+      const uint4 b = p.drop.on ? drop_bits(p.drop, off, row, g) : make_uint4(0, 0, 0, 0);
       float v[8];
-      unpack8<TYPE>(v, ring[slot][0][t]);
+      unpack8<TYPE>(v, first());
       if constexpr (ACT != kActNone) {
         float w[8];
-        unpack8<TYPE>(w, ring[slot][1][t]);
+        unpack8<TYPE>(w, second());
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= act_slope<ACT>(w[j]);
+        for (int j = 0; j < 8; j += 2)
+          split2(mul2(pair2(v[j], v[j + 1]), act_slope2<ACT>(pair2(w[j], w[j + 1]))), v[j], v[j + 1]);
       }
       if (p.drop.on) drop8(v, p.drop, b);
-      if (p.dZ) storen<TYPE, 8>(v, p.dZ, (size_t)r * p.lddz + c, c, p.M, vd);
+      if (p.dZ) put8<TYPE>(v, d, c, p.M);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sum[j] += v[j];
-    }
+      for (int j = 0; j < 8; j += 2)
+        split2(add2(pair2(sum[j], sum[j + 1]), pair2(v[j], v[j + 1])), sum[j], sum[j + 1]);
+    });
   }
   if (!p.dbias) return;   // the same for the whole cluster
   __syncthreads();
@@ -156,21 +188,24 @@ int log2_up(int n, int most) {
 template <int TYPE, int ACT>
 cudaError_t launch_act_grad_typed(const ActGradArgs& a) {
   const int groups = (a.M + 7) / 8;
-  // Column groups per CTA (32 to 128 columns) and CTAs per cluster: four CTAs fit an SM,
-  // and what counts is that the last round over the SMs is full.
+  // Columns per CTA (16 to 128) and CTAs per cluster.  What counts, measured over all
+  // pairs at nine shapes, is about 4.6 CTAs per SM (2048 x 11008, gelu: 27.8 us with 86
+  // slabs x 8 against 33 us with 172 x 3 and 39 us with 688 x 3), four rows per thread
+  // (300 x 11008: 7.3 us with 86 x 4, 9.3 us with 86 x 8) and rows of whole 128-byte
+  // lines; clusters of 16 pay for narrow matrices alone (16384 x 64: 7.8 against 12 us;
+  // 8192 x 1024: 19.7 against 17.2 us).
+  static const double kLines[5] = {0, 0.75, 0.9, 0.98, 1.0};
   int lx = log2_up(groups, 4), S = 1;
   double best = 0;
-  for (int l = std::min(lx, 2); l <= std::min(lx, 4); ++l)
-    for (int k = 1; k <= 8; ++k) {
-      if (k > 1 && (long)a.N <= (long)(k - 1) * (kThreads >> l)) break;   // a CTA without rows
-      const long slabs = (groups + (1 << l) - 1) >> l, ctas = slabs * k, sms = a.num_sms;
-      const long room = 4 * sms, rounds = (ctas + room - 1) / room;
-      const long last = ctas - (rounds - 1) * room;
-      const double busy = (double)ctas / ((rounds - 1) * room + (last + sms - 1) / sms * sms);
-      const double cols = (double)groups / (slabs << l);
-      const double score = busy * cols * std::min(1.0, (double)ctas / (3 * sms)) * (l == 2 ? 0.9 : 1.0);
-      if (score > best * 1.01) best = score, lx = l, S = k;
+  for (int l = std::min(lx, 4); l >= std::min(lx, 1); --l) {
+    const long slabs = (groups + (1 << l) - 1) >> l;
+    const int ty = kThreads >> l;
+    for (int k = 1; k <= (l <= 1 ? 16 : 8) && (k == 1 || (k - 1) * ty < a.N); ++k) {
+      const double fill = std::min(1.0, slabs * k / (4.6 * a.num_sms)), depth = std::min(1.0, a.N / (4.0 * ty * k));
+      const double score = fill * std::sqrt(depth) * kLines[std::max(l, 1)] * groups / (slabs << l);
+      if (score > best * 1.005) best = score, lx = l, S = k;
     }
+  }
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -182,6 +217,10 @@ cudaError_t launch_act_grad_typed(const ActGradArgs& a) {
   cfg.stream = a.stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  if (S > 8) {   // clusters above the portable size
+    const cudaError_t e = cudaFuncSetAttribute(act_grad_kernel<TYPE, ACT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+  }
   return cudaLaunchKernelEx(&cfg, act_grad_kernel<TYPE, ACT>, a, lx, vec_rows(a.dY, a.lddy), vec_rows(a.Z, a.ldz),
                             vec_rows(a.dZ, a.lddz));
 }

@@ -362,8 +362,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 *unit(st.buf + kEpiBuf, lane, j) = pack8<TYPE>(v[0]);
                 *unit(st.buf + kEpiBuf, lane, j + 1) = pack8<TYPE>(v[1]);
               }
-#pragma unroll
-              for (int i = 0; i < 16; ++i) v[i >> 3][i & 7] = act_fwd<ACT>(v[i >> 3][i & 7]);
+              act_fwd_n<ACT, 8>(v[0]);
+              act_fwd_n<ACT, 8>(v[1]);
               if (p.e.drop.on) {
                 drop8(v[0], p.e.drop, drop_bits(p.e.drop, off, row, c >> 3));
                 drop8(v[1], p.e.drop, drop_bits(p.e.drop, off, row, (c >> 3) + 1));
