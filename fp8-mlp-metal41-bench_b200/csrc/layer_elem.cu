@@ -189,20 +189,24 @@ template <int TYPE, int ACT>
 cudaError_t launch_act_grad_typed(const ActGradArgs& a) {
   const int groups = (a.M + 7) / 8;
   // Columns per CTA (16 to 128) and CTAs per cluster.  What counts, measured over all
-  // pairs at nine shapes, is about 4.6 CTAs per SM (2048 x 11008, gelu: 27.8 us with 86
-  // slabs x 8 against 33 us with 172 x 3 and 39 us with 688 x 3), four rows per thread
-  // (300 x 11008: 7.3 us with 86 x 4, 9.3 us with 86 x 8) and rows of whole 128-byte
-  // lines; clusters of 16 pay for narrow matrices alone (16384 x 64: 7.8 against 12 us;
-  // 8192 x 1024: 19.7 against 17.2 us).
-  static const double kLines[5] = {0, 0.75, 0.9, 0.98, 1.0};
+  // pairs at nine shapes: SMs with equal numbers of CTAs, three or four each (2048 x 11008
+  // with dropout: 35.2 us with 86 slabs x 8 = 4.65 per SM, 41.6 us with 86 x 4 = 2.3),
+  // four rows per thread (300 x 11008: 7.3 us with 86 x 4, 9.3 us with 86 x 8) and rows
+  // of whole 128-byte lines (8192 x 1024: 17 us with 32 slabs x 8, 20 us with 64 x 8);
+  // clusters of 16 pay for narrow matrices alone (16384 x 64: 7.8 against 12 us), and
+  // sizes between the powers of two do not (172 x 6: 38.2 us).
+  static const double kLines[5] = {0, 0.6, 0.9, 0.98, 1.0};
   int lx = log2_up(groups, 4), S = 1;
   double best = 0;
   for (int l = std::min(lx, 4); l >= std::min(lx, 1); --l) {
-    const long slabs = (groups + (1 << l) - 1) >> l;
+    const long slabs = (groups + (1 << l) - 1) >> l, sms = a.num_sms;
     const int ty = kThreads >> l;
-    for (int k = 1; k <= (l <= 1 ? 16 : 8) && (k == 1 || (k - 1) * ty < a.N); ++k) {
-      const double fill = std::min(1.0, slabs * k / (4.6 * a.num_sms)), depth = std::min(1.0, a.N / (4.0 * ty * k));
-      const double score = fill * std::sqrt(depth) * kLines[std::max(l, 1)] * groups / (slabs << l);
+    const int most = slabs * 8 <= sms / 2 ? 16 : 8;
+    for (int k = 1; k <= most && (k == 1 || k / 2 * ty < a.N); k *= 2) {
+      const long ctas = slabs * k;
+      const double even = (double)ctas / ((ctas + sms - 1) / sms * sms);
+      const double fill = std::min(1.0, ctas / (3.5 * sms)), depth = std::min(1.0, a.N / (4.0 * ty * k));
+      const double score = even * std::sqrt(fill * depth) * kLines[std::max(l, 1)] * groups / (slabs << l);
       if (score > best * 1.005) best = score, lx = l, S = k;
     }
   }
