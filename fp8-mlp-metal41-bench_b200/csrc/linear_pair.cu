@@ -1,6 +1,4 @@
 // linear_pair.cu -- the layer's products for many tiles: persistent CTA pairs.
-#include <cstring>
-
 #include "linear.cuh"
 
 namespace mlpg {
@@ -8,33 +6,36 @@ namespace mlpg {
 namespace {
 
 // ---- CTA pairs ------------------------------------------------------------------------
-// 256 x BN tiles: each CTA holds 128 rows of the accumulator, loads its own rows of the
+// 256 x 256 tiles: each CTA holds 128 rows of the accumulator, loads its own rows of the
 // row operand and half of the columns of the column operand; the leader issues
 // tcgen05.mma.cta_group::2 over both CTAs' shared memory.
 //   warp 0      TMA producer, both CTAs
 //   warp 1      TMEM allocation; MMA issuer in the leader
-//   warps 4-11  epilogue: TMEM lane quadrant w % 4, one half of the columns each
+//   warps 4-19  epilogue: TMEM lane quadrant w % 4, 64 columns each
+// Sixteen epilogue warps, because an epilogue with an activation and dropout issues some
+// 40 instructions per element, and with eight warps their latencies showed: 2048 x 512 x
+// 11008 with gelu, dropout and residual 55 us against @@ us.
 //
 // F32 results (dW alone): the tensor cores cut low bits when they add to an
 // accumulator, about 2^-25 of it per step of 16, which grows with the contraction
 // (measured against 64 bits: 6e-7 after 512, 5e-6 after 4096).  So every 512 deep the
-// partial sum leaves TMEM and is added in registers, rounded to nearest; the tile is
-// 128 columns wide there to leave room for 64 sums per thread.  16-bit results, whose
-// own rounding is 2^-12 or 2^-9, keep one accumulation.
-constexpr int kPairThreads = 384;
-constexpr int kEpiBuf = 4096;      // staging of 32 rows x 128 bytes
+// partial sum leaves TMEM and is added in registers, rounded to nearest.  16-bit results,
+// whose own rounding is 2^-12 or 2^-9, keep one accumulation.
+constexpr int kPairThreads = 640;
+constexpr int kEpiWarps = 16;
+constexpr int kEpiBuf = 4096;      // a warp's staging: 32 rows x 128 bytes
 constexpr int kGroupRows = 8;      // row tiles per group of the tile order
+constexpr int kSegment = 8;        // F32: stages per partial sum
 
-template <int OP, bool F32>
+template <int OP>
 struct PairCfg {
   static constexpr bool A_MN = OP == kOpDw, B_MN = OP != kOpDx;
-  static constexpr int BN = F32 ? 128 : 256, BH = BN / 2;
-  static constexpr int STAGES = F32 ? 6 : 5;
+  static constexpr int BN = 256, BH = BN / 2;
+  static constexpr int STAGES = 5;
   static constexpr int A_BYTES = 128 * 128, B_BYTES = BH * 128;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int SEG = 8;     // F32: stages per partial sum
   static constexpr int EPI_OFF = STAGES * STAGE_BYTES;
-  static constexpr int BAR_OFF = EPI_OFF + 8 * 2 * kEpiBuf;
+  static constexpr int BAR_OFF = EPI_OFF + kEpiWarps * kEpiBuf;
   static constexpr int SMEM = BAR_OFF + 512 + 1024;
   static constexpr uint32_t TMEM_COLS = 2 * BN;
   static constexpr uint32_t IDESC = (1u << 4) | ((A_MN ? 1u : 0u) << 15) | ((B_MN ? 1u : 0u) << 16) |
@@ -45,7 +46,7 @@ struct PairCfg {
 struct PairBars {
   uint64_t full[8], empty[8];
   uint64_t acc_full[2], acc_empty[2];
-  uint64_t res[8][2];      // a warp's residual tile has landed
+  uint64_t res[kEpiWarps];      // a warp's residual tile has landed
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -104,36 +105,41 @@ __device__ __forceinline__ void copy_tile(unsigned char* st, void* g, long ld, i
     }
 }
 
-// A warp's staging buffers: tiles go out by TMA store (or plain stores), the residual
+// A warp's staging buffer: tiles go out by TMA store (or plain stores), the residual
 // comes in by TMA load (or plain loads) into the buffer that its result replaces.
 struct Staging {
-  unsigned char* buf;      // two of kEpiBuf
-  uint64_t* bar;           // two
-  uint32_t phase;          // bit b: parity of bar[b]'s next completion
+  unsigned char* buf;
+  uint64_t* bar;
+  uint32_t phase;          // parity of the bar's next completion
 };
 
 __device__ __forceinline__ uint4* unit(unsigned char* st, int row, int u) {
   return reinterpret_cast<uint4*>(st + row * 128 + ((u ^ (row & 7)) << 4));
 }
 
+// The stores before it have read the buffer.
+__device__ __forceinline__ void staging_free() {
+  if ((threadIdx.x & 31) == 0) bulk_wait_read_all();
+  __syncwarp();
+}
+
 template <bool F32>
-__device__ __forceinline__ void res_fetch(Staging& s, int b, const PairArgs& p, const CUtensorMap* m, int row0, int c0) {
+__device__ __forceinline__ void res_fetch(Staging& s, const PairArgs& p, const CUtensorMap* m, int row0, int c0) {
   if (p.res_tma) {
     if ((threadIdx.x & 31) == 0) {
-      mbar_arrive_expect_tx(&s.bar[b], kEpiBuf);
-      tma_load_2d(s.buf + b * kEpiBuf, m, &s.bar[b], c0, row0);
+      mbar_arrive_expect_tx(s.bar, kEpiBuf);
+      tma_load_2d(s.buf, m, s.bar, c0, row0);
     }
   } else {
-    copy_tile<false>(s.buf + b * kEpiBuf, const_cast<void*>(p.e.res), p.e.ldr, F32 ? 4 : 2, row0,
-                     c0, p.e.rows, p.e.cols);
+    copy_tile<false>(s.buf, const_cast<void*>(p.e.res), p.e.ldr, F32 ? 4 : 2, row0, c0, p.e.rows, p.e.cols);
   }
 }
 
-__device__ __forceinline__ bool res_wait(Staging& s, int b, const PairArgs& p, const AbortCtl& ctl) {
+__device__ __forceinline__ bool res_wait(Staging& s, const PairArgs& p, const AbortCtl& ctl) {
   bool ok = true;
   if (p.res_tma) {
-    ok = mbar_wait(&s.bar[b], (s.phase >> b) & 1u, ctl, 0x500 + b);
-    s.phase ^= 1u << b;
+    ok = mbar_wait(s.bar, s.phase, ctl, 0x500);
+    s.phase ^= 1u;
   }
   ok = __all_sync(0xffffffffu, ok);
   __syncwarp();
@@ -162,7 +168,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     linear_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                        const __grid_constant__ CUtensorMap tmOut, const __grid_constant__ CUtensorMap tmRes,
                        const __grid_constant__ CUtensorMap tmPre, const __grid_constant__ PairArgs p) {
-  using C = PairCfg<OP, F32>;
+  using C = PairCfg<OP>;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -171,7 +177,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   const uint32_t rank = cluster_ctarank();
   const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
   const int num_tiles = p.tiles_r * p.tiles_c;
-  const int seg = F32 ? C::SEG : p.num_kb;
+  const int seg = F32 ? kSegment : p.num_kb;
   AbortCtl ctl{p.e.dev_err, &bars->abort_flag};
 
   if (threadIdx.x == 0) {
@@ -181,10 +187,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&bars->acc_full[b], 1);
-      mbar_init(&bars->acc_empty[b], 2 * 8);   // the epilogue warps of both CTAs
+      mbar_init(&bars->acc_empty[b], 2 * kEpiWarps);   // the epilogue warps of both CTAs
     }
-    for (int w = 0; w < 8; ++w)
-      for (int b = 0; b < 2; ++b) mbar_init(&bars->res[w][b], 1);
+    for (int w = 0; w < kEpiWarps; ++w) mbar_init(&bars->res[w], 1);
     bars->abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tmA);
@@ -248,129 +253,113 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     aborted_any = !ok;
   } else if (warp >= 4) {
     const int q = warp & 3, h = (warp - 4) >> 2;
-    Staging st{smem + C::EPI_OFF + (warp - 4) * 2 * kEpiBuf, bars->res[warp - 4], 0u};
+    Staging st{smem + C::EPI_OFF + (warp - 4) * kEpiBuf, &bars->res[warp - 4], 0u};
     const uint64_t off = drop_offset(p.e.drop);
     int local = 0;
     bool ok = true;
-    constexpr int GC = F32 ? 32 : 64;            // columns per staged tile: 128 bytes
-    constexpr int NG = C::BH / GC;               // two staged tiles per warp and tile
-    static_assert(NG == 2, "two staging buffers");
     for (int t = pair; t < num_tiles && ok; t += npairs) {
       int tr, tc;
       tile_at(t, p, tr, tc);
-      const int row0 = tr * 256 + (int)rank * 128 + q * 32, c0 = tc * C::BN + h * C::BH;
-      const int row = row0 + lane;
-      const bool live0 = row0 < p.e.rows && c0 < p.e.cols, live1 = row0 < p.e.rows && c0 + GC < p.e.cols;
-      // with Z both buffers of a group are in use (0: Y, 1: Z), else groups alternate
-      const bool two = OP == kOpLinear && p.e.pre != nullptr;
-      const uint32_t quad = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(h * C::BH);
-      // the previous tile's stores have read the buffers; the residual's tiles come
-      // while the product is still running
-      if (lane == 0) bulk_wait_read_all();
-      __syncwarp();
-      if (p.e.res && live0) {
-        res_fetch<F32>(st, 0, p, &tmRes, row0, c0);
-        if (!two && live1) res_fetch<F32>(st, 1, p, &tmRes, row0, c0 + GC);
-      }
+      const int row0 = tr * 256 + (int)rank * 128 + q * 32, c0 = tc * C::BN + h * 64;
+      const bool live = row0 < p.e.rows && c0 < p.e.cols;
+      const bool pre = OP == kOpLinear && p.e.pre != nullptr;
+      const uint32_t quad = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(h * 64);
+      staging_free();
+      // the residual comes while the product is still running (Z has the buffer first)
+      if (live && p.e.res && !pre) res_fetch<F32>(st, p, &tmRes, row0, c0);
       auto release = [&](int buf) {
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster_relaxed(mapa_shared(&bars->acc_empty[buf], 0));
       };
+      auto acquire = [&](int buf) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars->acc_full[buf], (uint32_t)(local >> 1) & 1u, ctl, 0x400 + buf));
+        tc_fence_after();
+        return ok;
+      };
       if constexpr (F32) {
-        float sum[C::BH] = {};
+        float sum[64] = {};
         for (int s0 = 0; s0 < p.num_kb; s0 += seg, ++local) {
           const int buf = local & 1;
-          ok = __all_sync(0xffffffffu, mbar_wait(&bars->acc_full[buf], (uint32_t)(local >> 1) & 1u, ctl, 0x400 + buf));
-          if (!ok) break;
-          tc_fence_after();
+          if (!acquire(buf)) break;
 #pragma unroll
-          for (int j = 0; j < C::BH; j += 32) {
-            uint32_t ra[32];
-            tmem_ld_32x32b_x32(quad + (uint32_t)(buf * C::BN + j), ra);
+          for (int j = 0; j < 64; j += 16) {
+            uint32_t ra[16];
+            tmem_ld_32x32b_x16(quad + (uint32_t)(buf * C::BN + j), ra);
             tmem_ld_wait();
-            if (j + 32 == C::BH) release(buf);
+            if (j == 48) release(buf);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) sum[j + i] += __uint_as_float(ra[i]);
+            for (int i = 0; i < 16; ++i) sum[j + i] += __uint_as_float(ra[i]);
           }
         }
         if (!ok) break;
+        // two staged tiles of 32 columns
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-          if (!(g ? live1 : live0)) continue;
-          unsigned char* sb = st.buf + g * kEpiBuf;
-          if (p.e.res && !(ok = res_wait(st, g, p, ctl))) break;
+        for (int g = 0; g < 2; ++g) {
+          const int cg = c0 + 32 * g;
+          if (!live || cg >= p.e.cols) continue;
+          if (g) {
+            staging_free();
+            if (p.e.res) res_fetch<F32>(st, p, &tmRes, row0, cg);
+          }
+          if (p.e.res && !(ok = res_wait(st, p, ctl))) break;
 #pragma unroll
           for (int u = 0; u < 8; ++u) {
-            float4 v = make_float4(sum[32 * g + 4 * u], sum[32 * g + 4 * u + 1], sum[32 * g + 4 * u + 2],
-                                   sum[32 * g + 4 * u + 3]);
-            float4* at = reinterpret_cast<float4*>(unit(sb, lane, u));
-            if (p.e.res) {
-              const float4 r = *at;
-              v = make_float4(v.x + r.x, v.y + r.y, v.z + r.z, v.w + r.w);
-            }
-            *at = v;
+            const float* v = sum + 32 * g + 4 * u;
+            float4* at = reinterpret_cast<float4*>(unit(st.buf, lane, u));
+            const float4 r = p.e.res ? *at : make_float4(0.f, 0.f, 0.f, 0.f);
+            *at = make_float4(v[0] + r.x, v[1] + r.y, v[2] + r.z, v[3] + r.w);
           }
-          tile_out(sb, p.out_tma, &tmOut, p.e.out, p.e.ldo, 4, row0, c0 + g * GC, p.e.rows, p.e.cols);
+          tile_out(st.buf, p.out_tma, &tmOut, p.e.out, p.e.ldo, 4, row0, cg, p.e.rows, p.e.cols);
         }
       } else {
         const int buf = local & 1;
-        ok = __all_sync(0xffffffffu, mbar_wait(&bars->acc_full[buf], (uint32_t)(local >> 1) & 1u, ctl, 0x400 + buf));
-        if (!ok) break;
+        if (!acquire(buf)) break;
         ++local;
-        tc_fence_after();
         const uint32_t acc = quad + (uint32_t)(buf * C::BN);
-        if (!live0) {
+        if (!live) {
           release(buf);
           continue;
         }
+        // Z and Y are two passes over the accumulator through the one staging buffer
 #pragma unroll 1
-        for (int g = 0; g < NG; ++g) {
-          if (g && !live1) {
-            release(buf);
-            break;
+        for (int pass = pre ? 0 : 1; pass < 2; ++pass) {
+          if (pass && pre) {
+            staging_free();
+            if (p.e.res) res_fetch<F32>(st, p, &tmRes, row0, c0);
           }
-          const int cg = c0 + g * GC, b = two ? 0 : g;
-          unsigned char* sb = st.buf + b * kEpiBuf;
-          if (two && g) {
-            if (lane == 0) bulk_wait_read_all();
-            __syncwarp();
-            if (p.e.res) res_fetch<F32>(st, 0, p, &tmRes, row0, cg);
-          }
-          if (p.e.res && !(ok = res_wait(st, b, p, ctl))) break;
+          if (pass && p.e.res && !(ok = res_wait(st, p, ctl))) break;
           // sixteen columns per step, the next sixteen on their way; with the type and the
-          // activation known, four branches that no lane diverges on are all that is left
+          // activation known, a few branches that no lane diverges on are all that is left
           // (with the type and the activation asked at run time a step of eight took
           // 450 cycles, most of them in branches)
           uint32_t ra[16];
-          tmem_ld_32x32b_x16(acc + (uint32_t)(g * GC), ra);
+          tmem_ld_32x32b_x16(acc, ra);
 #pragma unroll 1
           for (int j = 0; j < 8; j += 2) {
             float v[2][8];
             tmem_ld_wait();
 #pragma unroll
             for (int i = 0; i < 16; ++i) v[i >> 3][i & 7] = __uint_as_float(ra[i]);
-            if (j < 6) tmem_ld_32x32b_x16(acc + (uint32_t)(g * GC + 8 * (j + 2)), ra);
-            else if (g == NG - 1) release(buf);
+            if (j < 6) tmem_ld_32x32b_x16(acc + (uint32_t)(8 * (j + 2)), ra);
+            else if (pass) release(buf);
+            uint4 *at0 = unit(st.buf, lane, j), *at1 = unit(st.buf, lane, j + 1);
             if constexpr (OP == kOpLinear) {
-              const int c = cg + 8 * j;
+              const int c = c0 + 8 * j;
               if (p.e.bias) {
                 add_bias8<TYPE>(v[0], p.e, c);
                 add_bias8<TYPE>(v[1], p.e, c + 8);
               }
-              if (two) {
-                *unit(st.buf + kEpiBuf, lane, j) = pack8<TYPE>(v[0]);
-                *unit(st.buf + kEpiBuf, lane, j + 1) = pack8<TYPE>(v[1]);
-              }
-              act_fwd_n<ACT, 8>(v[0]);
-              act_fwd_n<ACT, 8>(v[1]);
-              if (p.e.drop.on) {
-                drop8(v[0], p.e.drop, drop_bits(p.e.drop, off, row, c >> 3));
-                drop8(v[1], p.e.drop, drop_bits(p.e.drop, off, row, (c >> 3) + 1));
+              if (pass) {
+                act_fwd_n<ACT, 8>(v[0]);
+                act_fwd_n<ACT, 8>(v[1]);
+                if (p.e.drop.on) {
+                  drop8(v[0], p.e.drop, drop_bits(p.e.drop, off, row0 + lane, c >> 3));
+                  drop8(v[1], p.e.drop, drop_bits(p.e.drop, off, row0 + lane, (c >> 3) + 1));
+                }
               }
             }
-            uint4 *at0 = unit(sb, lane, j), *at1 = unit(sb, lane, j + 1);
-            if (p.e.res) {
+            if (p.e.res && pass) {
               float r[2][8];
               unpack8<TYPE>(r[0], *at0);
               unpack8<TYPE>(r[1], *at1);
@@ -380,8 +369,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             *at0 = pack8<TYPE>(v[0]);
             *at1 = pack8<TYPE>(v[1]);
           }
-          tile_out(sb, p.out_tma, &tmOut, p.e.out, p.e.ldo, 2, row0, cg, p.e.rows, p.e.cols);
-          if (two) tile_out(st.buf + kEpiBuf, p.pre_tma, &tmPre, p.e.pre, p.e.ldz, 2, row0, cg, p.e.rows, p.e.cols);
+          if (pass) tile_out(st.buf, p.out_tma, &tmOut, p.e.out, p.e.ldo, 2, row0, c0, p.e.rows, p.e.cols);
+          else tile_out(st.buf, p.pre_tma, &tmPre, p.e.pre, p.e.ldz, 2, row0, c0, p.e.rows, p.e.cols);
         }
       }
     }
@@ -405,7 +394,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 
 template <int OP, int TYPE, bool F32, int ACT>
 cudaError_t launch_one(const LinearArgs& a, const Operand& x, const Operand& y) {
-  using C = PairCfg<OP, F32>;
+  using C = PairCfg<OP>;
   PairArgs p = {};
   p.e = epilogue(a);
   p.tiles_r = (a.rows + 255) / 256;
