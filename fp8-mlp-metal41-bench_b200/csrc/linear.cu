@@ -1,5 +1,8 @@
 // linear.cu -- the layer's products: which kernel runs a call, and operands that the
 // TMA cannot read.
+#include <algorithm>
+#include <cmath>
+
 #include "linear.cuh"
 
 namespace mlpg {
@@ -50,19 +53,52 @@ struct Plan {
   int split;   // cluster size
 };
 
+// CTAs of clusters of S that are resident at once on a B200's 148 SMs (the occupancy
+// query's answers), one CTA per SM and two.
+constexpr int kRoom[2][kMaxSplit] = {{148, 148, 135, 132, 130, 132, 105, 120}, {296, 296, 279, 284, 280, 270, 259, 264}};
+
+// An estimate of the split kernel's time in us: loads bound by the busiest SM (91 GB/s) or
+// by HBM (6.6 TB/s, less with fewer CTAs than SMs), then the sums over the cluster and the
+// epilogue.  The constants are a fit to 99 products of 1 .. 4096 rows, every bn and
+// cluster size timed: the choice is on average 1.2 % slower than the best of them and at
+// most 14 %.
+double split_time(const LinearArgs& a, int bn, int S) {
+  const int per_sm = bn <= 64 ? 2 : 1, room = kRoom[per_sm - 1][S - 1];
+  const long num_kb = (a.depth + kKb - 1) / kKb, kb = (num_kb + S - 1) / S;
+  const long ctas = (long)((a.rows + bn - 1) / bn) * ((a.cols + 127) / 128) * S;
+  const double on_sm = (double)((ctas * per_sm + room - 1) / room), rounds = (double)((ctas + room - 1) / room);
+  const double load = on_sm * kb * (128 + bn) * 128e-6 / 0.0914;
+  const double hbm = ((double)a.rows + a.cols) * num_kb * kKb * 2e-6 / 6.6 * (1 + 0.67 * std::max(0.0, 1 - ctas / 160.0));
+  const double n = std::min(bn, a.rows);
+  const double sums = S > 1 ? (0.304 + n * 0.0172 * (S - 1) / S) * std::pow(on_sm, 1.14) : 0;
+  return 3.30 + std::max(load, hbm) + sums + n / S * 0.0183 * on_sm + n * 0.0053 + (rounds - 1) * 1.12;
+}
+
+// The same for the pair kernel: rounds of tiles over the pairs, or HBM.
+double pair_time(const LinearArgs& a) {
+  const long num_kb = (a.depth + kKb - 1) / kKb;
+  const long tiles = (long)((a.rows + 255) / 256) * ((a.cols + 255) / 256), pairs = a.num_sms / 2;
+  const double rounds = (double)((tiles + pairs - 1) / pairs);
+  const double hbm = ((double)a.rows + a.cols) * num_kb * kKb * 2e-6 / 6.3 + (double)a.rows * a.cols * 2e-6 / 5.0;
+  return 3.51 + std::max(rounds * std::max(num_kb * 0.367, 0.25) + 2.66, hbm);
+}
+
 Plan plan(const LinearArgs& a) {
-  if (a.out_type == kTypeF32) return {0, 1};
+  Plan best = {0, 1};
+  if (a.out_type == kTypeF32) return best;   // sums in registers: the pair kernel's
+  double t = pair_time(a);
   const int num_kb = (a.depth + kKb - 1) / kKb;
-  const long tiles_c = (a.cols + 127) / 128;
-  const long pair_tiles = (long)((a.rows + 255) / 256) * ((a.cols + 255) / 256);
-  if (a.rows > 256 && pair_tiles * 2 >= a.num_sms / 2) return {0, 1};
-  int bn = a.op == kOpDw ? 64 : 16;
-  while (bn < 256 && bn < a.rows) bn *= 2;
-  const long tiles = tiles_c * ((a.rows + bn - 1) / bn);
-  const long slots = (long)a.num_sms * (bn <= 64 ? 2 : 1);
-  int S = 1;
-  while (S < kMaxSplit && tiles * (S + 1) <= slots && num_kb >= 2 * (S + 1)) ++S;
-  return {bn, S};
+  for (int bn = a.op == kOpDw ? 64 : 16; bn <= 256; bn *= 2) {
+    const long tiles = (long)((a.rows + bn - 1) / bn) * ((a.cols + 127) / 128);
+    if (16L * bn < a.rows) continue;   // the fit's range: up to 16 row tiles, 3 CTAs per SM where split
+    for (int S = 1; S <= std::min({kMaxSplit, num_kb, bn == 256 ? 4 : kMaxSplit}); ++S) {
+      if (S > 1 && tiles * S > 3L * a.num_sms) break;
+      const double u = split_time(a, bn, S);
+      if (u < t) t = u, best = {bn, S};
+    }
+    if (bn >= a.rows) break;
+  }
+  return best;
 }
 
 }  // namespace
