@@ -57,21 +57,23 @@ struct Plan {
 // query's answers), one CTA per SM and two.
 constexpr int kRoom[2][kMaxSplit] = {{148, 148, 135, 132, 130, 132, 105, 120}, {296, 296, 279, 284, 280, 270, 259, 264}};
 
-// An estimate of the split kernel's time in us: loads bound by the busiest SM (91 GB/s) or
-// by HBM (6.6 TB/s, less with fewer CTAs than SMs), then the sums over the cluster and the
-// epilogue.  The constants are a fit to 99 products of 1 .. 4096 rows, every bn and
-// cluster size timed: the choice is on average 1.2 % slower than the best of them and at
-// most 14 %.
+// An estimate of the split kernel's time in us: loads bound by the busiest SM (103 GB/s,
+// 71 where a single CTA of a kind that shares its SM keeps but half of the bytes in
+// flight), by L2 (13.3 TB/s) or by HBM (6.6 TB/s, less with fewer CTAs than SMs), then the
+// sums over the cluster and the epilogue.  The constants are a fit to 99 products of
+// 1 .. 4096 rows, every bn and cluster size timed: the choice is on average 1.2 % slower
+// than the best of them and at most 18 %.
 double split_time(const LinearArgs& a, int bn, int S) {
-  const int per_sm = bn <= 64 ? 2 : 1, room = kRoom[per_sm - 1][S - 1];
+  const int per_sm = bn <= 128 ? 2 : 1, room = kRoom[per_sm - 1][S - 1];
   const long num_kb = (a.depth + kKb - 1) / kKb, kb = (num_kb + S - 1) / S;
   const long ctas = (long)((a.rows + bn - 1) / bn) * ((a.cols + 127) / 128) * S;
   const double on_sm = (double)((ctas * per_sm + room - 1) / room), rounds = (double)((ctas + room - 1) / room);
-  const double load = on_sm * kb * (128 + bn) * 128e-6 / 0.0914;
-  const double hbm = ((double)a.rows + a.cols) * num_kb * kKb * 2e-6 / 6.6 * (1 + 0.67 * std::max(0.0, 1 - ctas / 160.0));
+  const double mb = kb * (128 + bn) * 128e-6;   // a CTA's operands
+  const double load = on_sm * mb / (on_sm == 1 && per_sm == 2 ? 0.0708 : 0.1029);
+  const double hbm = ((double)a.rows + a.cols) * num_kb * kKb * 2e-6 / 6.6 * (1 + 0.37 * std::max(0.0, 1 - ctas / 160.0));
   const double n = std::min(bn, a.rows);
-  const double sums = S > 1 ? (0.304 + n * 0.0172 * (S - 1) / S) * std::pow(on_sm, 1.14) : 0;
-  return 3.30 + std::max(load, hbm) + sums + n / S * 0.0183 * on_sm + n * 0.0053 + (rounds - 1) * 1.12;
+  const double sums = S > 1 ? (0.338 + n * 0.0262 * (S - 1) / S) * std::pow(on_sm, 0.55) : 0;
+  return 2.91 + std::max({load, ctas * mb / 13.3, hbm}) + sums + n / S * 0.0177 * on_sm + n * 0.0028 + (rounds - 1) * 1.70;
 }
 
 // The same for the pair kernel: rounds of tiles over the pairs, or HBM.
@@ -80,7 +82,7 @@ double pair_time(const LinearArgs& a) {
   const long tiles = (long)((a.rows + 255) / 256) * ((a.cols + 255) / 256), pairs = a.num_sms / 2;
   const double rounds = (double)((tiles + pairs - 1) / pairs);
   const double hbm = ((double)a.rows + a.cols) * num_kb * kKb * 2e-6 / 6.3 + (double)a.rows * a.cols * 2e-6 / 5.0;
-  return 3.51 + std::max(rounds * std::max(num_kb * 0.367, 0.25) + 2.66, hbm);
+  return 3.54 + std::max(rounds * std::max(num_kb * 0.371, 0.08) + 2.64, hbm);
 }
 
 Plan plan(const LinearArgs& a) {

@@ -20,9 +20,9 @@ struct SplitCfg {
   static constexpr bool C_MN = OP != kOpDx, R_MN = OP == kOpDw;
   static constexpr int C_BYTES = 128 * 128, R_BYTES = BN * 128;
   static constexpr int STAGE_BYTES = C_BYTES + R_BYTES;
-  // BN <= 64: two CTAs per SM, about 100 KB each in flight
-  static constexpr int STAGES = BN <= 32 ? 5 : (BN == 64 ? 4 : (BN == 128 ? 6 : 4));
-  static constexpr int PER_SM = BN <= 64 ? 2 : 1;
+  // BN <= 128: two CTAs per SM, about 100 KB each in flight
+  static constexpr int STAGES = BN <= 32 ? 5 : (BN == 128 ? 3 : 4);
+  static constexpr int PER_SM = BN <= 128 ? 2 : 1;
   static constexpr int BAR_OFF = STAGES * STAGE_BYTES;
   static constexpr int SMEM = BAR_OFF + 512 + 1024;
   static constexpr uint32_t TMEM_COLS = BN < 32 ? 32 : BN;
@@ -82,6 +82,13 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<OP, BN>::PER_SM)
   const int kb0 = (int)((long)num_kb * rank / S), kb1 = (int)((long)num_kb * (rank + 1) / S);   // kb1 > kb0: S <= num_kb
   AbortCtl ctl{p.dev_err, &bars->abort_flag};
 
+  auto load_stage = [&](uint32_t stage, int kb) {
+    unsigned char* dst = smem + stage * C::STAGE_BYTES;
+    mbar_arrive_expect_tx(&bars->full[stage], C::STAGE_BYTES);
+    load_op<C::C_MN>(dst, &tmC, &bars->full[stage], c0, kb, 128);
+    load_op<C::R_MN>(dst + C::C_BYTES, &tmR, &bars->full[stage], r0, kb, BN);
+  };
+  const int first = min(C::STAGES, kb1 - kb0);   // stages that the ring takes at once
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
       mbar_init(&bars->full[s], 1);
@@ -90,8 +97,9 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<OP, BN>::PER_SM)
     mbar_init(&bars->acc, 1);
     bars->abort_flag = 0;
     fence_mbar_init();
-    tma_prefetch_desc(&tmC);
-    tma_prefetch_desc(&tmR);
+    fence_proxy_async_smem();
+    // the first loads leave before the CTA has its TMEM
+    for (int s = 0; s < first; ++s) load_stage((uint32_t)s, kb0 + s);
   }
   if (warp == 1) {
     tmem_alloc(&bars->tmem_base, C::TMEM_COLS);
@@ -106,13 +114,10 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<OP, BN>::PER_SM)
   float* part = reinterpret_cast<float*>(smem);   // [row][128 columns], over the drained ring
 
   if (warp == 0 && lane == 0) {
-    uint32_t stage = 0, phase = 0;
-    for (int kb = kb0; kb < kb1; ++kb) {
-      if (!mbar_wait(&bars->empty[stage], phase ^ 1u, ctl, 0x100 + stage)) { aborted_any = true; break; }
-      unsigned char* dst = smem + stage * C::STAGE_BYTES;
-      mbar_arrive_expect_tx(&bars->full[stage], C::STAGE_BYTES);
-      load_op<C::C_MN>(dst, &tmC, &bars->full[stage], c0, kb, 128);
-      load_op<C::R_MN>(dst + C::C_BYTES, &tmR, &bars->full[stage], r0, kb, BN);
+    uint32_t stage = 0, phase = 0;   // the ring's second round
+    for (int kb = kb0 + first; kb < kb1; ++kb) {
+      if (!mbar_wait(&bars->empty[stage], phase, ctl, 0x100 + stage)) { aborted_any = true; break; }
+      load_stage(stage, kb);
       if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
     }
   } else if (warp == 1 && lane == 0) {
