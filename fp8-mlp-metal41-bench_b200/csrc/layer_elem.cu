@@ -100,7 +100,9 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(const __grid_constant
   __shared__ uint4 ring[kDepth * (RES ? 2 : 1) * kThreads];
   const int t = (int)threadIdx.x;
   const int g = (int)(blockIdx.x << lx) + (t & ((1 << lx) - 1)), c = 8 * g;
+  griddep_launch();
   if (c >= p.M) return;
+  griddep_wait();
   const uint64_t off = drop_offset(p.drop);
   const int rows = (int)gridDim.y * (kThreads >> lx), r = (int)blockIdx.y * (kThreads >> lx) + (t >> lx);
   Walk y = walk(p.Y, p.ldy, vy, r, rows, c, p.M);
@@ -133,6 +135,7 @@ __global__ void __launch_bounds__(kThreads, 4) act_grad_kernel(const __grid_cons
   const int S = (int)gridDim.y, rank = (int)blockIdx.y;   // the cluster is the grid's y
   const int g = (int)(blockIdx.x << lx) + (t & (tx - 1)), c = 8 * g;
   float sum[8] = {};
+  griddep_wait();
   if (c < p.M) {
     const uint64_t off = drop_offset(p.drop);
     const int rows = S * ty, r = rank * ty + (t >> lx);
@@ -157,6 +160,7 @@ __global__ void __launch_bounds__(kThreads, 4) act_grad_kernel(const __grid_cons
         split2(add2(pair2(sum[j], sum[j + 1]), pair2(v[j], v[j + 1])), sum[j], sum[j + 1]);
     });
   }
+  griddep_launch();
   if (!p.dbias) return;   // the same for the whole cluster
   __syncthreads();
 #pragma unroll
@@ -211,7 +215,7 @@ cudaError_t launch_act_grad_typed(const ActGradArgs& a) {
     }
   }
   cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 1;
   attr[0].val.clusterDim.y = S;
@@ -220,7 +224,9 @@ cudaError_t launch_act_grad_typed(const ActGradArgs& a) {
   cfg.blockDim = dim3(kThreads);
   cfg.stream = a.stream;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.numAttrs = 2;
   if (S > 8) {   // clusters above the portable size
     const cudaError_t e = cudaFuncSetAttribute(act_grad_kernel<TYPE, ACT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
@@ -250,14 +256,18 @@ cudaError_t launch_dropout(const DropoutArgs& a) {
   const long most = std::max(1L, 6L * a.num_sms / slabs);
   const dim3 grid((unsigned)slabs, (unsigned)std::min({((long)a.N + ty - 1) / ty, most, 65535L}));
   const bool vx = vec_rows(a.X, a.ldx), vr = vec_rows(a.res, a.ldr), vy = vec_rows(a.Y, a.ldy);
-  if (a.type == kTypeF16) {
-    if (a.res) dropout_kernel<kTypeF16, true><<<grid, kThreads, 0, a.stream>>>(a, lx, vx, vr, vy);
-    else dropout_kernel<kTypeF16, false><<<grid, kThreads, 0, a.stream>>>(a, lx, vx, vr, vy);
-  } else {
-    if (a.res) dropout_kernel<kTypeBF16, true><<<grid, kThreads, 0, a.stream>>>(a, lx, vx, vr, vy);
-    else dropout_kernel<kTypeBF16, false><<<grid, kThreads, 0, a.stream>>>(a, lx, vx, vr, vy);
-  }
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = a.stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  auto kernel = a.type == kTypeF16 ? (a.res ? dropout_kernel<kTypeF16, true> : dropout_kernel<kTypeF16, false>)
+                                   : (a.res ? dropout_kernel<kTypeBF16, true> : dropout_kernel<kTypeBF16, false>);
+  return cudaLaunchKernelEx(&cfg, kernel, a, lx, vx, vr, vy);
 }
 
 cudaError_t launch_act_grad(const ActGradArgs& a) {

@@ -49,8 +49,9 @@ cudaError_t pack(Operand& o, unsigned char*& ws, const LinearArgs& a) {
 
 // Which kernel, and how it cuts the work.
 struct Plan {
-  int bn;      // 0: CTA pairs; else rows per CTA of the split kernel
+  int bn;      // 0: CTA pairs; else rows per tile of the split kernel
   int split;   // cluster size
+  int tiles;   // tiles per cluster
 };
 
 // CTAs of clusters of S that are resident at once on a B200's 148 SMs (the occupancy
@@ -63,10 +64,10 @@ constexpr int kRoom[2][kMaxSplit] = {{148, 148, 135, 132, 130, 132, 105, 120}, {
 // sums over the cluster and the epilogue.  The constants are a fit to 99 products of
 // 1 .. 4096 rows, every bn and cluster size timed: the choice is on average 1.2 % slower
 // than the best of them and at most 18 %.
-double split_time(const LinearArgs& a, int bn, int S) {
-  const int per_sm = bn <= 128 ? 2 : 1, room = kRoom[per_sm - 1][S - 1];
-  const long num_kb = (a.depth + kKb - 1) / kKb, kb = (num_kb + S - 1) / S;
-  const long ctas = (long)((a.rows + bn - 1) / bn) * ((a.cols + 127) / 128) * S;
+double split_time(const LinearArgs& a, int bn, int S, int T) {
+  const int per_sm = bn > 32 && bn <= 128 ? 2 : 1, room = kRoom[per_sm - 1][S - 1];
+  const long num_kb = (a.depth + kKb - 1) / kKb, kb = (num_kb * T + S - 1) / S;
+  const long ctas = ((long)((a.rows + bn - 1) / bn) * ((a.cols + 127) / 128) + T - 1) / T * S;
   const double on_sm = (double)((ctas * per_sm + room - 1) / room), rounds = (double)((ctas + room - 1) / room);
   const double mb = kb * (128 + bn) * 128e-6;   // a CTA's operands
   const double load = on_sm * mb / (on_sm == 1 && per_sm == 2 ? 0.0708 : 0.1029);
@@ -86,7 +87,7 @@ double pair_time(const LinearArgs& a) {
 }
 
 Plan plan(const LinearArgs& a) {
-  Plan best = {0, 1};
+  Plan best = {0, 1, 1};
   if (a.out_type == kTypeF32) return best;   // sums in registers: the pair kernel's
   double t = pair_time(a);
   const int num_kb = (a.depth + kKb - 1) / kKb;
@@ -95,8 +96,12 @@ Plan plan(const LinearArgs& a) {
     if (16L * bn < a.rows) continue;   // the fit's range: up to 16 row tiles, 3 CTAs per SM where split
     for (int S = 1; S <= std::min({kMaxSplit, num_kb, bn == 256 ? 4 : kMaxSplit}); ++S) {
       if (S > 1 && tiles * S > 3L * a.num_sms) break;
-      const double u = split_time(a, bn, S);
-      if (u < t) t = u, best = {bn, S};
+      const double u = split_time(a, bn, S, 1);
+      if (u < t) t = u, best = {bn, S, 1};
+    }
+    if (bn <= 32 && num_kb >= 3) {   // three CTAs on two tiles
+      const double u = split_time(a, bn, 3, 2);
+      if (u < t) t = u, best = {bn, 3, 2};
     }
     if (bn >= a.rows) break;
   }
@@ -118,7 +123,7 @@ cudaError_t launch_linear(const LinearArgs& a) {
   cudaError_t e;
   if ((e = pack(x, ws, a)) != cudaSuccess || (e = pack(y, ws, a)) != cudaSuccess) return e;
   const Plan pl = plan(a);
-  return pl.bn ? launch_split(a, x, y, pl.bn, pl.split) : launch_pair(a, x, y);
+  return pl.bn ? launch_split(a, x, y, pl.bn, pl.split, pl.tiles) : launch_pair(a, x, y);
 }
 
 }  // namespace mlpg

@@ -202,6 +202,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   tc_fence_before();
   cluster_sync();
   tc_fence_after();
+  griddep_wait();
+  griddep_launch();
   const uint32_t tmem_base = bars->tmem_base;
   bool aborted_any = false;
 
@@ -413,17 +415,19 @@ cudaError_t launch_one(const LinearArgs& a, const Operand& x, const Operand& y) 
   if (ok && p.pre_tma) ok = map_rows(&tmZ, a.pre, a.ldz, a.rows, a.cols, 2, 32);
   if (!ok) return cudaErrorInvalidValue;
   cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.blockDim = dim3(kPairThreads);
   cfg.gridDim = dim3(a.num_sms / 2 * 2);
   cfg.dynamicSmemBytes = C::SMEM;
   cfg.stream = a.stream;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   static Once once;
   int pairs = 0;
   auto k = linear_pair_kernel<OP, TYPE, F32, ACT>;

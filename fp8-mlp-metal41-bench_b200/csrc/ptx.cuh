@@ -41,6 +41,15 @@ __device__ __forceinline__ bool aborted(const AbortCtl& c) {
   return *reinterpret_cast<volatile int*>(c.smem_abort) != 0;
 }
 
+// ---- dependent launches ----------------------------------------------------------
+// The layer's kernels are launched with programmatic stream serialisation: a kernel may
+// be set up while the one before it in the stream still runs, and griddep_wait returns
+// when that one has completed and its writes are visible.  Nothing that another kernel
+// may have written is read, and nothing is written to global memory, before it.
+__device__ __forceinline__ void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// lets the next kernel be set up (it still waits for this one's end)
+__device__ __forceinline__ void griddep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // ---- mbarrier ----------------------------------------------------------------
 __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));

@@ -177,7 +177,8 @@ def linear_ref(x, w, bias, res, act, p, seed, offset):
 
 SIZES = [(1, 1, 1), (1, 64, 8), (2, 4096, 264), (3, 7, 5), (13, 520, 1000), (16, 129, 24), (17, 100, 33),
          (40, 64, 136), (65, 72, 257), (128, 512, 256), (130, 257, 264), (200, 1000, 520), (257, 640, 1032),
-         (700, 96, 2056), (1100, 520, 1288), (1300, 136, 2056), (1030, 77, 2571), (2310, 1160, 1112), (4200, 64, 808)]
+         (700, 96, 2056), (1100, 520, 1288), (1300, 136, 2056), (1030, 77, 2571), (2310, 1160, 1112), (4200, 64, 808), (3, 264, 10000), (31, 1090, 10112),
+         (16, 192, 11008), (9, 4104, 4096)]
 
 
 @pytest.mark.gpu
@@ -284,7 +285,7 @@ def test_linear_specials_stay_in_their_rows(gemm, N, M):
 
 
 GRAD_SIZES = [(1, 1, 1), (1, 264, 136), (5, 9, 7), (16, 520, 1032), (33, 257, 129), (64, 128, 128), (130, 1000, 264),
-              (333, 136, 2056), (600, 520, 520), (1050, 72, 200), (2100, 256, 264), (1300, 2056, 1288), (1029, 2571, 1101), (520, 2312, 1544), (65, 2600, 2056)]
+              (333, 136, 2056), (600, 520, 520), (1050, 72, 200), (2100, 256, 264), (1300, 2056, 1288), (1029, 2571, 1101), (520, 2312, 1544), (65, 2600, 2056), (5, 10240, 328), (32, 11008, 200)]
 
 
 @pytest.mark.gpu
