@@ -49,32 +49,31 @@ cudaError_t pack(Operand& o, unsigned char*& ws, const LinearArgs& a) {
 
 // Which kernel, and how it cuts the work.
 struct Plan {
-  int bn;      // 0: CTA pairs; else rows per tile of the split kernel
+  int bn;      // 0: CTA pairs; else rows per CTA of the split kernel
   int split;   // cluster size
-  int tiles;   // tiles per cluster
 };
 
 // CTAs of clusters of S that are resident at once on a B200's 148 SMs (the occupancy
 // query's answers), one CTA per SM and two.
 constexpr int kRoom[2][kMaxSplit] = {{148, 148, 135, 132, 130, 132, 105, 120}, {296, 296, 279, 284, 280, 270, 259, 264}};
 
-// An estimate of the split kernel's time in us: loads bound by the busiest SM (103 GB/s,
-// 71 where a single CTA of a kind that shares its SM keeps but half of the bytes in
-// flight), by L2 (13.3 TB/s) or by HBM (6.6 TB/s, less with fewer CTAs than SMs), then the
-// sums over the cluster and the epilogue.  The constants are a fit to 99 products of
-// 1 .. 4096 rows, every bn and cluster size timed: the choice is on average 1.2 % slower
-// than the best of them and at most 18 %.
-double split_time(const LinearArgs& a, int bn, int S, int T) {
-  const int per_sm = bn > 32 && bn <= 128 ? 2 : 1, room = kRoom[per_sm - 1][S - 1];
-  const long num_kb = (a.depth + kKb - 1) / kKb, kb = (num_kb * T + S - 1) / S;
-  const long ctas = ((long)((a.rows + bn - 1) / bn) * ((a.cols + 127) / 128) + T - 1) / T * S;
+// An estimate of the split kernel's time in us in a stream of such calls: loads bound by the
+// busiest SM (102 GB/s, 77 where a single CTA of a kind that shares its SM keeps but half
+// of the bytes in flight, 0.6 us per block at 256 rows) or by HBM (6.6 TB/s, less with
+// fewer CTAs than SMs), then the sums over the cluster and the epilogue.  The constants are
+// a fit to 99 products of 1 .. 4096 rows, every bn and cluster size timed: the choice is on
+// average 1.4 % slower than the best of them and at most 21 %.
+double split_time(const LinearArgs& a, int bn, int S) {
+  const int per_sm = bn <= 128 ? 2 : 1, room = kRoom[per_sm - 1][S - 1];
+  const long num_kb = (a.depth + kKb - 1) / kKb, kb = (num_kb + S - 1) / S;
+  const long ctas = (long)((a.rows + bn - 1) / bn) * ((a.cols + 127) / 128) * S;
   const double on_sm = (double)((ctas * per_sm + room - 1) / room), rounds = (double)((ctas + room - 1) / room);
-  const double mb = kb * (128 + bn) * 128e-6;   // a CTA's operands
-  const double load = on_sm * mb / (on_sm == 1 && per_sm == 2 ? 0.0708 : 0.1029);
-  const double hbm = ((double)a.rows + a.cols) * num_kb * kKb * 2e-6 / 6.6 * (1 + 0.37 * std::max(0.0, 1 - ctas / 160.0));
+  const double mb = (128 + bn) * 128e-6;   // a block of both operands
+  const double block = std::max(mb / (on_sm == 1 && per_sm == 2 ? 0.0772 : 0.1021), bn * 0.00238);
+  const double hbm = ((double)a.rows + a.cols) * num_kb * kKb * 2e-6 / 6.6 * (1 + 0.496 * std::max(0.0, 1 - ctas / 160.0));
   const double n = std::min(bn, a.rows);
-  const double sums = S > 1 ? (0.338 + n * 0.0262 * (S - 1) / S) * std::pow(on_sm, 0.55) : 0;
-  return 2.91 + std::max({load, ctas * mb / 13.3, hbm}) + sums + n / S * 0.0177 * on_sm + n * 0.0028 + (rounds - 1) * 1.70;
+  const double sums = S > 1 ? (0.267 + n * 0.0154 * (S - 1) / S) * std::pow(on_sm, 0.57) : 0;
+  return 2.54 + std::max(on_sm * kb * block, hbm) + sums + n / S * 0.0152 * on_sm + n * 0.0053 + (rounds - 1) * 3.13;
 }
 
 // The same for the pair kernel: rounds of tiles over the pairs, or HBM.
@@ -83,25 +82,21 @@ double pair_time(const LinearArgs& a) {
   const long tiles = (long)((a.rows + 255) / 256) * ((a.cols + 255) / 256), pairs = a.num_sms / 2;
   const double rounds = (double)((tiles + pairs - 1) / pairs);
   const double hbm = ((double)a.rows + a.cols) * num_kb * kKb * 2e-6 / 6.3 + (double)a.rows * a.cols * 2e-6 / 5.0;
-  return 3.54 + std::max(rounds * std::max(num_kb * 0.371, 0.08) + 2.64, hbm);
+  return 2.77 + std::max(rounds * std::max(num_kb * 0.337, 1.19) + 3.79, hbm);
 }
 
 Plan plan(const LinearArgs& a) {
-  Plan best = {0, 1, 1};
+  Plan best = {0, 1};
   if (a.out_type == kTypeF32) return best;   // sums in registers: the pair kernel's
   double t = pair_time(a);
   const int num_kb = (a.depth + kKb - 1) / kKb;
   for (int bn = a.op == kOpDw ? 64 : 16; bn <= 256; bn *= 2) {
     const long tiles = (long)((a.rows + bn - 1) / bn) * ((a.cols + 127) / 128);
-    if (16L * bn < a.rows) continue;   // the fit's range: up to 16 row tiles, 3 CTAs per SM where split
+    if (16L * bn < a.rows) continue;   // the fit's range: up to 16 row tiles, 4 CTAs per SM where split
     for (int S = 1; S <= std::min({kMaxSplit, num_kb, bn == 256 ? 4 : kMaxSplit}); ++S) {
-      if (S > 1 && tiles * S > 3L * a.num_sms) break;
-      const double u = split_time(a, bn, S, 1);
-      if (u < t) t = u, best = {bn, S, 1};
-    }
-    if (bn <= 32 && num_kb >= 3) {   // three CTAs on two tiles
-      const double u = split_time(a, bn, 3, 2);
-      if (u < t) t = u, best = {bn, 3, 2};
+      if (S > 1 && tiles * S > 4L * a.num_sms) break;
+      const double u = split_time(a, bn, S);
+      if (u < t) t = u, best = {bn, S};
     }
     if (bn >= a.rows) break;
   }
@@ -123,7 +118,7 @@ cudaError_t launch_linear(const LinearArgs& a) {
   cudaError_t e;
   if ((e = pack(x, ws, a)) != cudaSuccess || (e = pack(y, ws, a)) != cudaSuccess) return e;
   const Plan pl = plan(a);
-  return pl.bn ? launch_split(a, x, y, pl.bn, pl.split, pl.tiles) : launch_pair(a, x, y);
+  return pl.bn ? launch_split(a, x, y, pl.bn, pl.split) : launch_pair(a, x, y);
 }
 
 }  // namespace mlpg

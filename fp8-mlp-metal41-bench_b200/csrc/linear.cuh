@@ -133,9 +133,7 @@ cudaError_t prepare(Once& once, Kernel k, int smem, cudaLaunchConfig_t& cfg, int
 // rows_op, cols_op: the stored operands whose rows or columns index the result's rows
 // and columns (A and B of LinearArgs, packed where they had to be)
 cudaError_t launch_pair(const LinearArgs& a, const Operand& rows_op, const Operand& cols_op);
-// bn rows per tile (16, 32, 64, 128, 256; dW from 64), clusters of `split` CTAs on `tiles`
-// tiles (1; 2 with bn <= 32)
-cudaError_t launch_split(const LinearArgs& a, const Operand& rows_op, const Operand& cols_op, int bn, int split,
-                         int tiles);
+// bn rows per CTA (16, 32, 64, 128, 256; dW from 64), clusters of `split`
+cudaError_t launch_split(const LinearArgs& a, const Operand& rows_op, const Operand& cols_op, int bn, int split);
 
 }  // namespace mlpg

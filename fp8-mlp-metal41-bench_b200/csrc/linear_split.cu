@@ -7,13 +7,12 @@ namespace mlpg {
 namespace {
 
 // ---- few rows -----------------------------------------------------------------------------
-// A cluster of S CTAs computes T tiles of 128 columns x BN rows, the columns as the MMA's
-// 128 lanes (so a single row still fills the tensor core's M and the epilogue's threads).
-// The T tiles' contractions, one behind the other, are cut into S equal runs, one per
-// CTA; each CTA puts its partial sums into its own shared memory, and each then sums and
-// finishes its share of the rows over distributed shared memory, in rank order: no
-// workspace, no atomics, the same result every time.  T is 1, or 2 where 1.5 CTAs per
-// tile fill the SMs and whole numbers do not (86 tiles: 129 CTAs of equal runs).
+// One CTA computes 128 columns x BN rows over its share of the contraction, with the
+// columns as the MMA's 128 lanes (so a single row still fills the tensor core's M and
+// the epilogue's threads).  The cluster's CTAs split the contraction, put their partial
+// sums into their own shared memory, and each then sums and finishes its share of the
+// tile over distributed shared memory, in rank order: no workspace, no atomics, the
+// same result every time.
 constexpr int kSplitThreads = 256;
 
 template <int OP, int BN>
@@ -21,23 +20,22 @@ struct SplitCfg {
   static constexpr bool C_MN = OP != kOpDx, R_MN = OP == kOpDw;
   static constexpr int C_BYTES = 128 * 128, R_BYTES = BN * 128;
   static constexpr int STAGE_BYTES = C_BYTES + R_BYTES;
-  // the weights' stream wants 180 KB in flight per SM: one CTA, or two where the rows'
-  // epilogue is long enough to hide behind the other's loads
-  static constexpr int STAGES = BN <= 32 ? 10 : (BN == 128 ? 3 : 4);
-  static constexpr int PER_SM = BN > 32 && BN <= 128 ? 2 : 1;
+  // BN <= 128: two CTAs per SM, about 100 KB each in flight (one CTA per SM with ten stages
+  // streams W more slowly: 1 x 4096 x 11008 18.8 against 16.5 us)
+  static constexpr int STAGES = BN <= 32 ? 5 : (BN == 128 ? 3 : 4);
+  static constexpr int PER_SM = BN <= 128 ? 2 : 1;
   static constexpr int BAR_OFF = STAGES * STAGE_BYTES;
   static constexpr int SMEM = BAR_OFF + 512 + 1024;
-  static constexpr int MAX_T = BN <= 32 ? 2 : 1;
-  static constexpr uint32_t TMEM_COLS = MAX_T * BN;
+  static constexpr uint32_t TMEM_COLS = BN < 32 ? 32 : BN;
   static constexpr uint32_t IDESC = (1u << 4) | ((C_MN ? 1u : 0u) << 15) | ((R_MN ? 1u : 0u) << 16) |
                                     ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-  static_assert(MAX_T * BN * 512 <= BAR_OFF, "partial sums fit the ring");
+  static_assert(BN * 512 <= BAR_OFF, "partial sums fit the ring");
   static_assert(SMEM * PER_SM <= kSmemMax, "shared memory budget");
   static_assert(!R_MN || BN % 64 == 0, "whole MN boxes");
 };
 
 struct SplitBars {
-  uint64_t full[10], empty[10], acc;
+  uint64_t full[8], empty[8], acc;
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -70,7 +68,7 @@ __device__ __forceinline__ uint32_t cluster_nctarank() {
 template <int OP, int TYPE, int BN>
 __global__ void __launch_bounds__(kSplitThreads, SplitCfg<OP, BN>::PER_SM)
     linear_split_kernel(const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmR,
-                        const __grid_constant__ EpiArgs p, int tiles, int T) {
+                        const __grid_constant__ EpiArgs p) {
   using C = SplitCfg<OP, BN>;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem =
@@ -79,26 +77,20 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<OP, BN>::PER_SM)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cluster_ctarank(), S = (int)cluster_nctarank();
   const int tiles_c = (p.cols + 127) / 128;
-  const int tile0 = (int)(blockIdx.x / S) * T;
+  const int tile = blockIdx.x / S;
+  const int c0 = tile % tiles_c * 128, r0 = tile / tiles_c * BN;
   const int num_kb = (p.depth + kKb - 1) / kKb;
-  // contraction blocks of the cluster's tiles in one row; this CTA's run (S <= num_kb)
-  // (num_kb <= 2^24: 32 bits hold the products)
-  const uint32_t units = (uint32_t)(num_kb * min(T, tiles - tile0));
-  const int u0 = (int)(units * (uint32_t)rank / (uint32_t)S), u1 = (int)(units * (uint32_t)(rank + 1) / (uint32_t)S);
-  const int tr0 = tile0 / tiles_c, tc0 = tile0 - tr0 * tiles_c;
-  const int wrap = tc0 + 1 == tiles_c;   // the second tile starts the next row of tiles
-  const int r0s[2] = {tr0 * BN, (tr0 + wrap) * BN}, c0s[2] = {tc0 * 128, wrap ? 0 : (tc0 + 1) * 128};
+  // this CTA's run of the contraction; not empty, S <= num_kb (<= 2^24: 32 bits hold the products)
+  const int kb0 = num_kb * rank / S, kb1 = num_kb * (rank + 1) / S;
   AbortCtl ctl{p.dev_err, &bars->abort_flag};
 
-  auto load_stage = [&](uint32_t stage, int u) {
-    const bool second = u >= num_kb;
-    const int kb = second ? u - num_kb : u, c0 = second ? c0s[1] : c0s[0], r0 = second ? r0s[1] : r0s[0];
+  auto load_stage = [&](uint32_t stage, int kb) {
     unsigned char* dst = smem + stage * C::STAGE_BYTES;
     mbar_arrive_expect_tx(&bars->full[stage], C::STAGE_BYTES);
     load_op<C::C_MN>(dst, &tmC, &bars->full[stage], c0, kb, 128);
     load_op<C::R_MN>(dst + C::C_BYTES, &tmR, &bars->full[stage], r0, kb, BN);
   };
-  const int first = min(C::STAGES, u1 - u0);   // stages that the ring takes at once
+  const int first = min(C::STAGES, kb1 - kb0);   // stages that the ring takes at once
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
       mbar_init(&bars->full[s], 1);
@@ -110,7 +102,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<OP, BN>::PER_SM)
     fence_proxy_async_smem();
     // the first loads leave before the CTA has its TMEM
     griddep_wait();
-    for (int s = 0; s < first; ++s) load_stage((uint32_t)s, u0 + s);
+    for (int s = 0; s < first; ++s) load_stage((uint32_t)s, kb0 + s);
   }
   if (warp == 1) {
     tmem_alloc(&bars->tmem_base, C::TMEM_COLS);
@@ -122,14 +114,14 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<OP, BN>::PER_SM)
   griddep_wait();
   const uint32_t tmem_base = bars->tmem_base;
   bool aborted_any = false;
-  float* part = reinterpret_cast<float*>(smem);   // [tile][row][128 columns], over the drained ring
-  auto tile_rows = [&](int j) { return min(BN, p.rows - (j ? r0s[1] : r0s[0])); };
+  const int nrows = min(BN, p.rows - r0);
+  float* part = reinterpret_cast<float*>(smem);   // [row][128 columns], over the drained ring
 
   if (warp == 0 && lane == 0) {
     uint32_t stage = 0, phase = 0;   // the ring's second round
-    for (int u = u0 + first; u < u1; ++u) {
+    for (int kb = kb0 + first; kb < kb1; ++kb) {
       if (!mbar_wait(&bars->empty[stage], phase, ctl, 0x100 + stage)) { aborted_any = true; break; }
-      load_stage(stage, u);
+      load_stage(stage, kb);
       if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
     }
   } else if (warp == 1 && lane == 0) {
@@ -137,17 +129,14 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<OP, BN>::PER_SM)
     const uint32_t smem_base = smem_u32(smem);
     constexpr uint32_t fmt = TYPE == kTypeBF16 ? 1u : 0u;
     const uint32_t idesc = C::IDESC | (fmt << 7) | (fmt << 10);
-    for (int u = u0; u < u1; ++u) {
+    for (int kb = kb0; kb < kb1; ++kb) {
       if (!mbar_wait(&bars->full[stage], phase, ctl, 0x300 + stage)) { aborted_any = true; break; }
       tc_fence_after();
-      // a tile's first block in this run starts its accumulator
-      const uint32_t d = tmem_base + (u >= num_kb ? (uint32_t)BN : 0u);
-      const bool fresh = u == u0 || u == num_kb;
       const uint32_t a = smem_base + stage * C::STAGE_BYTES, b = a + C::C_BYTES;
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk)
-        tc_mma<kKindF16>(d, op_desc(a, C::C_MN, kk), op_desc(b, C::R_MN, kk), idesc,
-                         (!fresh || kk != 0) ? 1u : 0u);
+        tc_mma<kKindF16>(tmem_base, op_desc(a, C::C_MN, kk), op_desc(b, C::R_MN, kk), idesc,
+                         (kb != kb0 || kk != 0) ? 1u : 0u);
       tc_commit(&bars->empty[stage]);
       if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
     }
@@ -159,21 +148,17 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<OP, BN>::PER_SM)
     aborted_any = !ok;
     if (ok) {
       tc_fence_after();
+      const uint32_t acc = tmem_base + ((uint32_t)(q * 32) << 16);
       constexpr int CH = BN < 32 ? 16 : 32;
 #pragma unroll 1
-      for (int j = u0 >= num_kb; j <= (u1 > num_kb); ++j) {   // the tiles of this run
-        const uint32_t acc = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(j * BN);
-        const int nrows = tile_rows(j);
-#pragma unroll 1
-        for (int n0 = 0; n0 < nrows; n0 += CH) {
-          uint32_t r[CH];
-          if constexpr (CH == 16) tmem_ld_32x32b_x16(acc + (uint32_t)n0, r);
-          else tmem_ld_32x32b_x32(acc + (uint32_t)n0, r);
-          tmem_ld_wait();
+      for (int n0 = 0; n0 < nrows; n0 += CH) {
+        uint32_t r[CH];
+        if constexpr (CH == 16) tmem_ld_32x32b_x16(acc + (uint32_t)n0, r);
+        else tmem_ld_32x32b_x32(acc + (uint32_t)n0, r);
+        tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < CH; ++i)
-            if (n0 + i < nrows) part[(j * BN + n0 + i) * 128 + q * 32 + lane] = __uint_as_float(r[i]);
-        }
+        for (int i = 0; i < CH; ++i)
+          if (n0 + i < nrows) part[(n0 + i) * 128 + q * 32 + lane] = __uint_as_float(r[i]);
       }
       tc_fence_before();
     }
@@ -183,7 +168,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<OP, BN>::PER_SM)
     while (global_ns() - t0 < 100000ull) {}
   }
   __syncwarp();
-  griddep_launch();
+  griddep_launch();   // not earlier: the next kernel's CTAs would fill this one's gaps unevenly
   if (S > 1) cluster_sync();
   else __syncthreads();
   if (warp == 1) {
@@ -191,34 +176,25 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<OP, BN>::PER_SM)
     tmem_dealloc(tmem_base, C::TMEM_COLS);
   }
 
-  // The tiles' rows go round the cluster.  A thread finishes four columns: the 32 lanes
+  // The tile's rows go round the cluster.  A thread finishes four columns: the 32 lanes
   // then read 512 contiguous bytes of each partial sum, which is what the SM-to-SM
   // network carries best (eight columns per thread, half of the lanes' 16-byte units at
   // a time, took twice as long).
   const uint64_t off = drop_offset(p.drop);
-#pragma unroll 1
-  for (int j = 0; j < T && tile0 + j < tiles; ++j) {
-    const int nrows = tile_rows(j), r0 = j ? r0s[1] : r0s[0], c = (j ? c0s[1] : c0s[0]) + 4 * lane;
-    if (c >= p.cols) continue;
-    // ranks whose runs touch the tile: consecutive ones
-    int s0 = 0, s1 = S;
-    if (T > 1) {
-      const uint32_t t0 = (uint32_t)(j * num_kb), t1 = t0 + (uint32_t)num_kb;
-      while (units * (uint32_t)(s0 + 1) < (t0 + 1) * (uint32_t)S) ++s0;   // that run ends at or before t0
-      while (units * (uint32_t)(s1 - 1) >= t1 * (uint32_t)S) --s1;        // that one starts at or behind t1
-    }
+  const int c = c0 + 4 * lane;
+  if (c < p.cols) {
     for (int n = rank + S * warp; n < nrows; n += S * (kSplitThreads / 32)) {
       const int row = r0 + n;
-      const uint32_t at = smem_u32(part) + (uint32_t)((j * BN + n) * 128 + 4 * lane) * 4u;
+      const uint32_t at = smem_u32(part) + (uint32_t)(n * 128 + 4 * lane) * 4u;
       // every partial sum's load is in flight before the first is added
       float4 x[kMaxSplit];
 #pragma unroll
       for (int s = 0; s < kMaxSplit; ++s)
-        if (s < s1 - s0) x[s] = ld_dsmem_f4(mapa_addr(at, (uint32_t)(s0 + s)));
+        if (s < S) x[s] = ld_dsmem_f4(mapa_addr(at, (uint32_t)s));
       float v[4] = {};
 #pragma unroll
       for (int s = 0; s < kMaxSplit; ++s)
-        if (s < s1 - s0) {
+        if (s < S) {
           v[0] += x[s].x;
           v[1] += x[s].y;
           v[2] += x[s].z;
@@ -251,7 +227,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<OP, BN>::PER_SM)
 }
 
 template <int OP, int TYPE, int BN>
-cudaError_t launch_one(const LinearArgs& a, const Operand& x, const Operand& y, int S, int T) {
+cudaError_t launch_one(const LinearArgs& a, const Operand& x, const Operand& y, int S) {
   using C = SplitCfg<OP, BN>;
   const EpiArgs p = epilogue(a);
   CUtensorMap tmC, tmR;
@@ -267,8 +243,7 @@ cudaError_t launch_one(const LinearArgs& a, const Operand& x, const Operand& y, 
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.blockDim = dim3(kSplitThreads);
-  const int tiles = (a.cols + 127) / 128 * ((a.rows + BN - 1) / BN);
-  cfg.gridDim = dim3((unsigned)((tiles + T - 1) / T) * S);
+  cfg.gridDim = dim3((unsigned)((a.cols + 127) / 128) * ((a.rows + BN - 1) / BN) * S);
   cfg.dynamicSmemBytes = C::SMEM;
   cfg.stream = a.stream;
   cfg.attrs = attr;
@@ -277,32 +252,32 @@ cudaError_t launch_one(const LinearArgs& a, const Operand& x, const Operand& y, 
   auto k = linear_split_kernel<OP, TYPE, BN>;
   cudaError_t e = prepare(once, k, C::SMEM, cfg, nullptr);
   if (e != cudaSuccess) return e;
-  return cudaLaunchKernelEx(&cfg, k, tmC, tmR, p, tiles, T);
+  return cudaLaunchKernelEx(&cfg, k, tmC, tmR, p);
 }
 
 template <int OP, int TYPE>
-cudaError_t launch_bn(const LinearArgs& a, const Operand& x, const Operand& y, int bn, int S, int T) {
+cudaError_t launch_bn(const LinearArgs& a, const Operand& x, const Operand& y, int bn, int S) {
   if constexpr (OP != kOpDw) {
-    if (bn == 16) return launch_one<OP, TYPE, 16>(a, x, y, S, T);
-    if (bn == 32) return launch_one<OP, TYPE, 32>(a, x, y, S, T);
+    if (bn == 16) return launch_one<OP, TYPE, 16>(a, x, y, S);
+    if (bn == 32) return launch_one<OP, TYPE, 32>(a, x, y, S);
   }
-  if (bn == 64) return launch_one<OP, TYPE, 64>(a, x, y, S, T);
-  if (bn == 128) return launch_one<OP, TYPE, 128>(a, x, y, S, T);
-  return launch_one<OP, TYPE, 256>(a, x, y, S, T);
+  if (bn == 64) return launch_one<OP, TYPE, 64>(a, x, y, S);
+  if (bn == 128) return launch_one<OP, TYPE, 128>(a, x, y, S);
+  return launch_one<OP, TYPE, 256>(a, x, y, S);
 }
 
 template <int TYPE>
-cudaError_t launch_typed(const LinearArgs& a, const Operand& x, const Operand& y, int bn, int S, int T) {
-  if (a.op == kOpLinear) return launch_bn<kOpLinear, TYPE>(a, x, y, bn, S, T);
-  if (a.op == kOpDx) return launch_bn<kOpDx, TYPE>(a, x, y, bn, S, T);
-  return launch_bn<kOpDw, TYPE>(a, x, y, bn, S, T);
+cudaError_t launch_typed(const LinearArgs& a, const Operand& x, const Operand& y, int bn, int S) {
+  if (a.op == kOpLinear) return launch_bn<kOpLinear, TYPE>(a, x, y, bn, S);
+  if (a.op == kOpDx) return launch_bn<kOpDx, TYPE>(a, x, y, bn, S);
+  return launch_bn<kOpDw, TYPE>(a, x, y, bn, S);
 }
 
 }  // namespace
 
-cudaError_t launch_split(const LinearArgs& a, const Operand& rows_op, const Operand& cols_op, int bn, int split, int tiles) {
-  return a.type == kTypeF16 ? launch_typed<kTypeF16>(a, rows_op, cols_op, bn, split, tiles)
-                            : launch_typed<kTypeBF16>(a, rows_op, cols_op, bn, split, tiles);
+cudaError_t launch_split(const LinearArgs& a, const Operand& rows_op, const Operand& cols_op, int bn, int split) {
+  return a.type == kTypeF16 ? launch_typed<kTypeF16>(a, rows_op, cols_op, bn, split)
+                            : launch_typed<kTypeBF16>(a, rows_op, cols_op, bn, split);
 }
 
 }  // namespace mlpg
