@@ -765,6 +765,7 @@ int run_product(int device, LinearArgs& a, int type, int out_type, const char* a
   if ((rc = check_matrix(bn, a.B, type, a.ldb, M))) return rc;
   if ((rc = check_matrix(on, out, out_type, ldo, a.cols))) return rc;
   if ((rc = check_matrix("residual", res, out_type, ldr, a.cols, true))) return rc;
+  if (out == a.A || out == a.B) return fail(GEMM_ERR_ARGS, "%s and an operand are the same buffer", on);
   a.type = type;
   a.out_type = out_type;
   a.out = out;
@@ -806,7 +807,8 @@ int gemm_linear(int device, int type, const void* X, long ldx, const void* W, lo
   if ((rc = make_dropout(&q.dropout, &a.drop))) return rc;
   if (q.bias && !elem_aligned(q.bias, type)) return fail(GEMM_ERR_ARGS, "bias is not aligned to its element");
   if ((rc = check_matrix("preact", q.preact, type, q.ldz, M, true))) return rc;
-  if (q.preact && q.preact == Y) return fail(GEMM_ERR_ARGS, "preact and Y are the same buffer");
+  if (q.preact && (q.preact == Y || q.preact == X || q.preact == W || q.preact == q.residual))
+    return fail(GEMM_ERR_ARGS, "preact and another operand are the same buffer");
   a.bias = q.bias;
   a.pre = q.preact;
   a.ldz = dense(q.ldz, M);

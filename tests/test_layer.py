@@ -48,13 +48,13 @@ def test_philox_known_answers():
         [0xD16CFE09, 0x94FDCCEB, 0x5001E420, 0x24126EA1]
 
 
-def factors(rows, cols, p, seed, offset):
-    """Dropout's factor of every element, [rows, cols] in 64 bits, from the generator in numpy."""
+def factors(rows, cols, p, seed, offset, first=0):
+    """Dropout's factor of every element of rows first .. first + rows - 1, in 64 bits, from the generator in numpy."""
     t = int(np.rint(p * 65536))
     groups = (cols + 7) // 8
     u = np.uint64
     c = [np.broadcast_to(np.arange(groups, dtype=u), (rows, groups)),
-         np.broadcast_to(np.arange(rows, dtype=u)[:, None], (rows, groups)),
+         np.broadcast_to(np.arange(first, first + rows, dtype=u)[:, None], (rows, groups)),
          np.full((rows, groups), offset & 0xFFFFFFFF, u), np.full((rows, groups), (offset >> 32) & 0xFFFFFFFF, u)]
     k = [seed & 0xFFFFFFFF, seed >> 32]
     m, s = u(0xFFFFFFFF), u(32)
@@ -178,7 +178,8 @@ def linear_ref(x, w, bias, res, act, p, seed, offset):
 SIZES = [(1, 1, 1), (1, 64, 8), (2, 4096, 264), (3, 7, 5), (13, 520, 1000), (16, 129, 24), (17, 100, 33),
          (40, 64, 136), (65, 72, 257), (128, 512, 256), (130, 257, 264), (200, 1000, 520), (257, 640, 1032),
          (700, 96, 2056), (1100, 520, 1288), (1300, 136, 2056), (1030, 77, 2571), (2310, 1160, 1112), (4200, 64, 808), (3, 264, 10000), (31, 1090, 10112),
-         (16, 192, 11008), (9, 4104, 4096)]
+         (16, 192, 11008), (9, 4104, 4096), (201, 40, 10023), (2200, 646, 40), (1124, 67, 43), (536, 66, 41),
+         (320, 144, 37)]
 
 
 @pytest.mark.gpu
@@ -285,7 +286,9 @@ def test_linear_specials_stay_in_their_rows(gemm, N, M):
 
 
 GRAD_SIZES = [(1, 1, 1), (1, 264, 136), (5, 9, 7), (16, 520, 1032), (33, 257, 129), (64, 128, 128), (130, 1000, 264),
-              (333, 136, 2056), (600, 520, 520), (1050, 72, 200), (2100, 256, 264), (1300, 2056, 1288), (1029, 2571, 1101), (520, 2312, 1544), (65, 2600, 2056), (5, 10240, 328), (32, 11008, 200)]
+              (333, 136, 2056), (600, 520, 520), (1050, 72, 200), (2100, 256, 264), (1300, 2056, 1288), (1029, 2571, 1101), (520, 2312, 1544), (65, 2600, 2056), (5, 10240, 328), (32, 11008, 200),
+              (200, 10012, 36), (2126, 34, 616), (1075, 43, 65), (1, 200, 9657), (646, 2259, 32), (68, 1119, 37),
+              (1, 1073, 33), (259, 34, 136)]
 
 
 @pytest.mark.gpu
@@ -471,6 +474,38 @@ def test_dropout_strided(gemm):
         assert bool((buf == 7.0).all())
 
 
+# ---- past 32 bits --------------------------------------------------------------------------------
+@pytest.mark.gpu
+def test_offsets_past_32_bits(gemm):
+    # 2.2e9 elements: the last rows lie behind 2^31 of them
+    N, M, K, t = 270001, 8200, 24, torch.bfloat16
+    x, w = rand((N, K), t, 1), rand((K, M), t, 2, K ** -0.5)
+    y = torch.empty(N, M, dtype=t, device="cuda")
+    G.linear(0, 1, x, w, y, N, K, M, act=G.ACTS["relu"], stream=stream())
+    G.sync(0, stream())
+    for lo, hi in ((0, 40), (N - 300, N)):
+        z = x[lo:hi].double() @ w.double()
+        v = act64(z, "relu")
+        assert_close(y[lo:hi], v, 1.2 * product_error(x[lo:hi], w, K) + half_step(v, t) * 1.01, "Y")
+    z = y[N - 300:].clone()
+    db = torch.empty(M, device="cuda")
+    G.act_grad(0, 1, y, y, y, db, N, M, act=G.ACTS["relu"], stream=stream())     # relu of a relu: y itself
+    G.dropout(0, 1, y, y, N, M, 0.5, 3, 4, stream=stream())
+    G.sync(0, stream())
+    f = torch.from_numpy(factors(300, M, 0.5, 3, 4, first=N - 300)).cuda()
+    assert torch.equal(y[N - 300:].double(), z.double() * f)
+    dw = torch.empty(K, M, device="cuda")
+    G.linear_dw(0, 1, x, y, dw, N, K, M, out_type=G.TYPES["f32"], stream=stream())
+    G.sync(0, stream())
+    ref = torch.zeros(K, M, dtype=torch.float64, device="cuda")
+    mag = torch.zeros_like(ref)
+    for i in range(0, N, 30000):
+        a, b = x[i:i + 30000].double(), y[i:i + 30000].double()
+        ref += a.t() @ b
+        mag += a.abs().t() @ b.abs()
+    assert_close(dw, ref, mag * ((512 / 16 + 16 + N / 512) * 2.0 ** -23) + half_step(ref, torch.float32), "dW")
+
+
 # ---- together -----------------------------------------------------------------------------------
 class Mlp:
     """x + D(W2 act(W1 x + b1) + b2), forward and backward through the C ABI."""
@@ -580,6 +615,103 @@ def test_two_streams_and_repeats_agree(gemm):
         assert all(torch.equal(a, b) for a, b in zip(o, outs[0]))
 
 
+@pytest.mark.gpu
+def test_fork_and_join_in_a_graph(gemm):
+    # kernels set up early wait for everything before them: a long product on a forked stream, joined, then read
+    N, K, M, t = 1536, 2048, 2048, torch.bfloat16
+    x, w, x2 = rand((N, K), t, 1), rand((K, M), t, 2, K ** -0.5), rand((N, K), t, 3)
+    a, b, c, y = (torch.zeros(N, M, dtype=t, device="cuda") for _ in range(4))
+    s, side = torch.cuda.Stream(), torch.cuda.Stream()
+
+    def step(wait=lambda: None):
+        cur = torch.cuda.current_stream()
+        G.linear(0, 1, x, w, a, N, K, M, stream=cur.cuda_stream)
+        wait()
+        side.wait_stream(cur)
+        with torch.cuda.stream(side):
+            G.linear(0, 1, x2, w, b, N, K, M, residual=a, stream=side.cuda_stream)
+            wait()
+            G.linear(0, 1, x2, w, b, N, K, M, residual=b, stream=side.cuda_stream)
+            wait()
+        G.dropout(0, 1, a, c, N, M, 0.0, 0, 0, stream=cur.cuda_stream)
+        wait()
+        cur.wait_stream(side)
+        G.dropout(0, 1, c, y, N, M, 0.5, 1, 2, residual=b, stream=cur.cuda_stream)
+
+    def run(call):
+        for v in (a, b, c, y):
+            v.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s):
+            call()
+        torch.cuda.synchronize()
+        return y.clone()
+
+    ref = run(lambda: step(torch.cuda.synchronize))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        step()
+    for _ in range(5):
+        assert torch.equal(run(step), ref) and torch.equal(run(g.replay), ref)
+
+
+@pytest.mark.gpu
+def test_chained_calls_see_each_other(gemm):
+    # a chain of small calls, each reading what the one before wrote, against the same chain with waits in between
+    N, d, t = 33, 264, torch.float16
+    w = rand((d, d), t, 1, d ** -0.5)
+    x0 = rand((N, d), t, 2)
+
+    def chain(wait):
+        bufs = [x0.clone(), torch.empty_like(x0)]
+        db = torch.empty(d, device="cuda")
+        for i in range(40):
+            a, b = bufs[i % 2], bufs[(i + 1) % 2]
+            if i % 3 == 0:
+                G.linear(0, 0, a, w, b, N, d, d, act=G.ACTS["silu"], residual=a, stream=stream())
+            elif i % 3 == 1:
+                G.dropout(0, 0, a, b, N, d, 0.1, i, 0, stream=stream())
+            else:
+                G.act_grad(0, 0, a, a, b, db, N, d, act=G.ACTS["gelu"], stream=stream())
+            if wait:
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        return bufs[0], db
+
+    ref = chain(True)
+    for _ in range(10):
+        assert all(torch.equal(u, v) for u, v in zip(chain(False), ref))
+
+
+@pytest.mark.gpu
+def test_two_host_threads(gemm):
+    import threading
+    N, K, M, t = 64, 1000, 520, torch.bfloat16
+    x, w = rand((N, K), t, 1), rand((K, M), t, 2, K ** -0.5)
+    outs, errors = {}, []
+
+    def work(i):
+        try:
+            s = torch.cuda.Stream()
+            o = torch.empty(N, M, dtype=t, device="cuda")
+            s.wait_stream(torch.cuda.default_stream())
+            for _ in range(200):
+                G.linear(0, 1, x, w, o, N, K, M, act=G.ACTS["gelu_tanh"], stream=s.cuda_stream)
+            G.sync(0, s.cuda_stream)
+            outs[i] = o
+        except Exception as e:   # noqa: BLE001 - reported below
+            errors.append(e)
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not errors
+    assert all(torch.equal(outs[i], outs[0]) for i in range(4))
+
+
 # ---- refusals (no GPU needed: arguments are checked before the device) -----------------------------
 P = 1 << 20   # stands for an aligned address; refused calls read nothing
 
@@ -597,24 +729,27 @@ def refused(call, *words):
     (dict(Y=None), "null Y"), (dict(N=0), "N=0"), (dict(K=-1), "K=-1"), (dict(M=(1 << 30) + 1), "M="),
     (dict(ldx=63), "X"), (dict(ldw=71), "W"), (dict(ldy=-72), "Y"), (dict(X=P + 1), "aligned"),
     (dict(Y=P + 1), "aligned"), (dict(bias=P + 1), "bias"), (dict(residual=P + 1), "residual"),
-    (dict(residual=P, ldr=8), "residual"), (dict(preact=P, ldz=8), "preact"), (dict(preact=P + 4096), "same buffer"),
+    (dict(residual=P, ldr=8), "residual"), (dict(Y=P), "same buffer"), (dict(preact=P), "same buffer"),
+    (dict(residual=P + 8192, preact=P + 8192), "same buffer"), (dict(preact=P, ldz=8), "preact"), (dict(preact=P + 4096), "same buffer"),
     (dict(act=5), "activation"), (dict(act=-1), "activation"), (dict(dropout_p=1.5), "probability"),
     (dict(dropout_p=-0.1), "probability"), (dict(dropout_p=float("nan")), "probability"),
     (dict(offset_ptr=P + 4), "offset_ptr")])
 def test_linear_refusals(kw, word):
-    a = dict(type=0, X=P, W=P, Y=P + 4096, N=4, K=64, M=72)
+    a = dict(type=0, X=P, W=P + 2048, Y=P + 4096, N=4, K=64, M=72)
     a.update(kw)
     refused(lambda: G.linear(0, **a), word)
 
 
 def test_gradient_product_refusals():
     refused(lambda: G.linear_dx(0, 2, P, P, P, 4, 64, 72), "type")
-    refused(lambda: G.linear_dx(0, 0, P, P, P, 4, 64, 72, lddz=71), "dZ")
-    refused(lambda: G.linear_dx(0, 0, P, P, P, 4, 64, 72, lddx=63), "dX")
+    refused(lambda: G.linear_dx(0, 0, P, P, P + 64, 4, 64, 72, lddz=71), "dZ")
+    refused(lambda: G.linear_dx(0, 0, P, P + 64, P, 4, 64, 72), "same buffer")
+    refused(lambda: G.linear_dw(0, 0, P, P + 64, P + 64, 4, 64, 72), "same buffer")
+    refused(lambda: G.linear_dx(0, 0, P, P, P + 64, 4, 64, 72, lddx=63), "dX")
     refused(lambda: G.linear_dx(0, 0, P, None, P, 4, 64, 72), "null W")
-    refused(lambda: G.linear_dw(0, 0, P, P, P, 4, 64, 72, out_type=1), "result type")
+    refused(lambda: G.linear_dw(0, 0, P, P, P + 64, 4, 64, 72, out_type=1), "result type")
     refused(lambda: G.linear_dw(0, 1, P, P, P + 2, 4, 64, 72, out_type=2), "aligned")
-    refused(lambda: G.linear_dw(0, 1, P, P, P, 4, 64, 72, out_type=2, residual=P, ldr=71), "residual")
+    refused(lambda: G.linear_dw(0, 1, P, P, P + 64, 4, 64, 72, out_type=2, residual=P + 64, ldr=71), "residual")
     refused(lambda: G.linear_dw(0, 1, P, None, P, 4, 64, 72), "null dZ")
 
 
@@ -638,8 +773,8 @@ def test_act_grad_and_dropout_refusals():
 def test_good_arguments_need_the_device():
     if G.device_count() > 0:
         pytest.skip("a GPU is present")
-    for call in (lambda: G.linear(0, 0, P, P, P + 4096, 4, 64, 72), lambda: G.linear_dx(0, 1, P, P, P, 4, 64, 72),
-                 lambda: G.linear_dw(0, 1, P, P, P, 4, 64, 72, out_type=2),
+    for call in (lambda: G.linear(0, 0, P, P, P + 4096, 4, 64, 72), lambda: G.linear_dx(0, 1, P, P, P + 4096, 4, 64, 72),
+                 lambda: G.linear_dw(0, 1, P, P, P + 4096, 4, 64, 72, out_type=2),
                  lambda: G.act_grad(0, 0, P, P, P, P, 4, 8, act=1), lambda: G.dropout(0, 0, P, P, 4, 8, 0.5, 0, 0),
                  lambda: G.linear(99, 0, P, P, P + 4096, 4, 64, 72)):
         with pytest.raises(G.GemmError) as e:
