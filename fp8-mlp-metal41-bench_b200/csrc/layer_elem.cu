@@ -100,7 +100,6 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(const __grid_constant
   __shared__ uint4 ring[kDepth * (RES ? 2 : 1) * kThreads];
   const int t = (int)threadIdx.x;
   const int g = (int)(blockIdx.x << lx) + (t & ((1 << lx) - 1)), c = 8 * g;
-  griddep_launch();
   if (c >= p.M) return;
   griddep_wait();
   const uint64_t off = drop_offset(p.drop);
@@ -121,6 +120,7 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(const __grid_constant
     }
     put8<TYPE>(v, y, c, p.M);
   });
+  griddep_launch();
 }
 
 // A cluster's CTAs share the rows of one slab of columns.  Each thread's eight column

@@ -146,9 +146,11 @@ __device__ __forceinline__ bool res_wait(Staging& s, const PairArgs& p, const Ab
   return ok;
 }
 
+// A TMA store clips at the map's last column in units of 16 bytes (measured: it fills the
+// unit with zeros), so a tile that holds a part of a unit goes out by plain stores.
 __device__ __forceinline__ void tile_out(unsigned char* st, bool tma, const CUtensorMap* m, void* g, long ld, int es,
                                          int row0, int c0, int rows, int cols) {
-  if (tma) {
+  if (tma && (c0 + 128 / es <= cols || ((unsigned)cols * es) % 16u == 0)) {
     fence_proxy_async_smem();
     __syncwarp();
     if ((threadIdx.x & 31) == 0) {
@@ -203,7 +205,6 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   cluster_sync();
   tc_fence_after();
   griddep_wait();
-  griddep_launch();
   const uint32_t tmem_base = bars->tmem_base;
   bool aborted_any = false;
 
@@ -386,6 +387,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     while (global_ns() - t0 < 100000ull) {}
   }
   __syncwarp();
+  // Not earlier: the next kernel's CTAs would crowd onto the SMs that the last, partial
+  // round of tiles leaves idle.
+  griddep_launch();
   tc_fence_before();
   cluster_sync();
   if (warp == 1) {

@@ -254,6 +254,39 @@ def test_linear_strides_and_alignment(gemm, N, M, pad, shift):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("N", [1, 21, 1290])
+def test_odd_rows_on_aligned_pitches(gemm, N):
+    # rows of odd length that start on 16 bytes: read and written in place, up to their last element and no further
+    K, M, ldk, ldm, t = 133, 2003, 136, 2008, torch.bfloat16
+    x0, w0, r0, dz0 = rand((N, K), t, 1), rand((K, M), t, 2, K ** -0.5), rand((N, M), t, 3), rand((N, M), t, 4)
+    x, w, r, dz = put(x0, ldk), put(w0, ldm), put(r0, ldm), put(dz0, ldm)
+    assert workspace(G.OP_LINEAR, x, w, N, K, M, ldk, ldm)[1] == 0
+    ybuf, y = strided((N, M), t, ldm, 0, 7.0)
+    zbuf, z = strided((N, M), t, ldm, 0, 7.0)
+    G.linear(0, 1, x, w, y, N, K, M, act=G.ACTS["silu"], residual=r, preact=z, dropout_p=0.2, seed=9, offset=1,
+             ldx=ldk, ldw=ldm, ldy=ldm, ldr=ldm, ldz=ldm, stream=stream())
+    xbuf, dx = strided((N, K), t, ldk, 0, 7.0)
+    G.linear_dx(0, 1, dz, w, dx, N, K, M, lddz=ldm, ldw=ldm, lddx=ldk, stream=stream())
+    wbufs = []
+    for out in ("bf16", "f32"):
+        wbufs.append(strided((K, M), ttype(out), ldm, 0, 7.0))
+        G.linear_dw(0, 1, x, dz, wbufs[-1][1], N, K, M, out_type=G.TYPES[out], ldx=ldk, lddz=ldm, lddw=ldm,
+                    stream=stream())
+    G.sync(0, stream())
+    ry, rz, ty, tz = linear_ref(x0, w0, None, r0, "silu", 0.2, 9, 1)
+    assert_close(y, ry, ty, "Y")
+    assert_close(z, rz, tz, "Z")
+    v = dz0.double() @ w0.double().t()
+    assert_close(dx, v, product_error(dz0, w0.t(), M) + half_step(v, t) * 1.01, "dX")
+    v = x0.double().t() @ dz0.double()
+    for _, dw in wbufs:
+        assert_close(dw, v, product_error(x0.t(), dz0, N) + half_step(v, dw.dtype) * 1.01, "dW")
+    for buf, view in [(ybuf, y), (zbuf, z), (xbuf, dx)] + wbufs:
+        view.fill_(7.0)
+        assert bool((buf == 7.0).all()), "an element between rows was written"
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("N,M", [(4, 272), (333, 272), (1300, 2056)])
 def test_linear_residual_in_place(gemm, N, M):
     K, t = 264, torch.bfloat16
@@ -616,6 +649,40 @@ def test_two_streams_and_repeats_agree(gemm):
 
 
 @pytest.mark.gpu
+def test_first_calls_of_a_process_may_be_captured():
+    # the kernels' one-time set-up needs no call before the capture
+    import os
+    import subprocess
+    import sys
+    code = f"""
+import sys
+sys.path.insert(0, {os.path.dirname(os.path.dirname(os.path.abspath(G.__file__)))!r})
+import torch
+from mlpgemm import lib as G
+G.init(0)
+t = torch.float16
+x, w, dz = (torch.randn(*s, device="cuda").to(t) for s in ((40, 1000), (1000, 1336), (40, 1336)))
+y, z = torch.empty_like(dz), torch.empty_like(dz)
+dx, dw, db = torch.empty_like(x), torch.empty(1000, 1336, device="cuda"), torch.empty(1336, device="cuda")
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    s = torch.cuda.current_stream().cuda_stream
+    G.linear(0, 0, x, w, y, 40, 1000, 1336, act=2, preact=z, dropout_p=0.1, seed=1, stream=s)
+    G.act_grad(0, 0, dz, z, z, db, 40, 1336, act=2, stream=s)
+    G.linear_dx(0, 0, z, w, dx, 40, 1000, 1336, stream=s)
+    G.linear_dw(0, 0, x, z, dw, 40, 1000, 1336, out_type=2, stream=s)
+    G.dropout(0, 0, y, y, 40, 1336, 0.5, 1, 2, stream=s)
+g.replay()
+torch.cuda.synchronize()
+ref = x.double().t() @ z.double()
+assert float((dw.double() - ref).norm() / ref.norm()) < 1e-6
+print("captured")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.gpu
 def test_fork_and_join_in_a_graph(gemm):
     # kernels set up early wait for everything before them: a long product on a forked stream, joined, then read
     N, K, M, t = 1536, 2048, 2048, torch.bfloat16
@@ -738,6 +805,14 @@ def test_linear_refusals(kw, word):
     a = dict(type=0, X=P, W=P + 2048, Y=P + 4096, N=4, K=64, M=72)
     a.update(kw)
     refused(lambda: G.linear(0, **a), word)
+
+
+def test_workspace_refusals():
+    need = G.linear_workspace(G.OP_LINEAR, P, P + 2048, 4, 63, 72)
+    assert need > 0
+    for ws, n, word in ((None, 0, "workspace"), (P + 65536, need - 1, "workspace"), (P + 65536 + 8, need, "aligned")):
+        refused(lambda: G.linear(0, 0, P, P + 2048, P + 4096, 4, 63, 72, workspace=ws, workspace_bytes=n), word)
+        refused(lambda: G.linear_dw(0, 0, P, P + 2048, P + 4096, 4, 63, 72, workspace=ws, workspace_bytes=n), word)
 
 
 def test_gradient_product_refusals():
