@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import subprocess
 import threading
 
@@ -42,17 +43,10 @@ ACTS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 OP_LINEAR, OP_DX, OP_DW = 0, 1, 2
 
 
-class DropoutArgs(ctypes.Structure):
-    """gemm_dropout_args"""
-    _fields_ = [("p", ctypes.c_double), ("seed", ctypes.c_uint64), ("offset", ctypes.c_uint64),
-                ("offset_ptr", ctypes.c_void_p)]
-
-
-class Epilogue(ctypes.Structure):
-    """gemm_epilogue"""
-    _fields_ = [("bias", ctypes.c_void_p), ("residual", ctypes.c_void_p), ("ldr", ctypes.c_long),
-                ("preact", ctypes.c_void_p), ("ldz", ctypes.c_long), ("act", ctypes.c_int),
-                ("dropout", DropoutArgs)]
+# gemm_dropout_args and gemm_epilogue, packed for one call (a few times cheaper than ctypes structures)
+DROPOUT_ARGS = struct.Struct("=dQQQ")                 # p, seed, offset, offset_ptr
+EPILOGUE = struct.Struct("=QQqQqi4xdQQQ")             # bias, residual, ldr, preact, ldz, act, dropout
+_U64 = (1 << 64) - 1
 
 
 class GemmError(RuntimeError):
@@ -142,6 +136,8 @@ def _declare(L):
 def lib() -> ctypes.CDLL:
     """Load libgemm.so (once).  Raises GemmError(GEMM_ERR_INIT) if it is absent."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is None:
             if not os.path.exists(LIB_PATH):
@@ -260,8 +256,8 @@ class DeviceBuffer:
 
 def as_ptr(x):
     """Device pointer of a DeviceBuffer, a torch tensor, an int or None."""
-    if x is None:
-        return None
+    if x is None or type(x) is int:
+        return x
     if isinstance(x, DeviceBuffer):
         return x.ptr
     if hasattr(x, "data_ptr"):
@@ -391,8 +387,8 @@ def quantize(device, fmt, src, dst, scales=None, rows=1, cols=1, stream=None) ->
 
 
 # ---- the MLP layer (f16 / bf16 operands; see the header for the formulas) -----------------
-def _dropout(p, seed, offset, offset_ptr) -> DropoutArgs:
-    return DropoutArgs(p, seed, offset, as_ptr(offset_ptr))
+def _dropout(p, seed, offset, offset_ptr) -> bytes:
+    return DROPOUT_ARGS.pack(p, seed & _U64, offset & _U64, as_ptr(offset_ptr) or 0)
 
 
 def linear_workspace(op: int, A, B, N: int, K: int, M: int, lda: int = 0, ldb: int = 0) -> int:
@@ -404,10 +400,10 @@ def linear(device, type, X, W, Y, N, K, M, bias=None, act=0, residual=None, prea
            offset=0, offset_ptr=None, ldx=0, ldw=0, ldy=0, ldr=0, ldz=0, workspace=None, workspace_bytes=0,
            stream=None) -> None:
     """Y = residual + dropout(act(X @ W + bias)); preact receives X @ W + bias.  Row lengths 0: dense."""
-    epi = Epilogue(as_ptr(bias), as_ptr(residual), ldr, as_ptr(preact), ldz, act,
-                   _dropout(dropout_p, seed, offset, offset_ptr))
+    epi = EPILOGUE.pack(as_ptr(bias) or 0, as_ptr(residual) or 0, ldr, as_ptr(preact) or 0, ldz, act, dropout_p,
+                        seed & _U64, offset & _U64, as_ptr(offset_ptr) or 0)
     check(lib().gemm_linear(device, type, as_ptr(X), ldx, as_ptr(W), ldw, as_ptr(Y), ldy, N, K, M,
-                            ctypes.addressof(epi), as_ptr(workspace), int(workspace_bytes), as_ptr(stream)),
+                            epi, as_ptr(workspace), int(workspace_bytes), as_ptr(stream)),
           "gemm_linear")
 
 
@@ -432,7 +428,7 @@ def act_grad(device, type, dY, Z, dZ, dbias, N, M, act=0, dropout_p=0.0, seed=0,
     """dZ = dropout(dY) * act'(Z); dbias (f32) = its column sums."""
     drop = _dropout(dropout_p, seed, offset, offset_ptr)
     check(lib().gemm_act_grad(device, type, as_ptr(dY), lddy, as_ptr(Z), ldz, as_ptr(dZ), lddz, as_ptr(dbias), N, M,
-                              act, ctypes.addressof(drop), as_ptr(stream)), "gemm_act_grad")
+                              act, drop, as_ptr(stream)), "gemm_act_grad")
 
 
 def dropout(device, type, X, Y, N, M, p, seed, offset, offset_ptr=None, residual=None, ldx=0, ldr=0, ldy=0,
@@ -440,4 +436,4 @@ def dropout(device, type, X, Y, N, M, p, seed, offset, offset_ptr=None, residual
     """Y = residual + dropout(X); on dY the same call is its gradient."""
     drop = _dropout(p, seed, offset, offset_ptr)
     check(lib().gemm_dropout(device, type, as_ptr(X), ldx, as_ptr(residual), ldr, as_ptr(Y), ldy, N, M,
-                             ctypes.addressof(drop), as_ptr(stream)), "gemm_dropout")
+                             drop, as_ptr(stream)), "gemm_dropout")

@@ -871,7 +871,18 @@ def test_workspace_is_for_operands_the_tma_cannot_read():
 
 
 def test_structures_match_the_header():
-    # x86-64 layout of the C structures
-    assert ctypes.sizeof(G.DropoutArgs) == 32
-    assert G.Epilogue.ldr.offset == 16 and G.Epilogue.act.offset == 40 and G.Epilogue.dropout.offset == 48
-    assert ctypes.sizeof(G.Epilogue) == 80
+    # the packed forms against C structures with the header's members (x86-64 layout)
+    class Drop(ctypes.Structure):
+        _fields_ = [("p", ctypes.c_double), ("seed", ctypes.c_uint64), ("offset", ctypes.c_uint64),
+                    ("offset_ptr", ctypes.c_void_p)]
+
+    class Epi(ctypes.Structure):
+        _fields_ = [("bias", ctypes.c_void_p), ("residual", ctypes.c_void_p), ("ldr", ctypes.c_long),
+                    ("preact", ctypes.c_void_p), ("ldz", ctypes.c_long), ("act", ctypes.c_int), ("dropout", Drop)]
+
+    assert G.DROPOUT_ARGS.size == ctypes.sizeof(Drop) and G.EPILOGUE.size == ctypes.sizeof(Epi)
+    e = Epi.from_buffer_copy(G.EPILOGUE.pack(1, 2, -3, 4, 5, 6, 0.75, 2 ** 64 - 1, 9, 10))
+    assert (e.bias, e.residual, e.ldr, e.preact, e.ldz, e.act) == (1, 2, -3, 4, 5, 6)
+    assert (e.dropout.p, e.dropout.seed, e.dropout.offset, e.dropout.offset_ptr) == (0.75, 2 ** 64 - 1, 9, 10)
+    d = Drop.from_buffer_copy(G.DROPOUT_ARGS.pack(0.5, 7, 8, 0))
+    assert (d.p, d.seed, d.offset, d.offset_ptr) == (0.5, 7, 8, None)
