@@ -20,28 +20,45 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// Rows whose 16-byte groups are aligned.
-bool vec_rows(const void* p, long ld) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && ld % 8 == 0; }
+// The widest unit (16, 8, 4 or 2 bytes) on which every row of a matrix starts.
+int row_unit(const void* p, long ld) {
+  const uint64_t x = reinterpret_cast<uintptr_t>(p) | (uint64_t)(2 * ld) | 16u;
+  return (int)(x & (~x + 1));
+}
 
 constexpr int kDepth = 4;
 
-// A thread's walk down its rows of one operand: the next row's address, and whether its
-// eight columns are one aligned 16-byte unit.
+// A thread's walk down its rows of one operand: the next row's address, and the unit in
+// which its eight columns are read or written (2 for a group that ends behind the row).
 struct Walk {
   const uint16_t* p;
   long step;      // elements from one of the thread's rows to the next
-  bool unit;
+  int unit;
 };
 
-__device__ __forceinline__ Walk walk(const void* base, long ld, bool vec, int r, int rows, int c, int cols) {
-  return Walk{static_cast<const uint16_t*>(base) + (size_t)r * ld + c, ld * rows, vec && c + 8 <= cols};
+__device__ __forceinline__ Walk walk(const void* base, long ld, int unit, int r, int rows, int c, int cols) {
+  return Walk{static_cast<const uint16_t*>(base) + (size_t)r * ld + c, ld * rows, c + 8 <= cols ? unit : 2};
 }
 
-// The walk's row to shared memory: cp.async where it is one unit, else plain loads, with
-// zeros past the row's end.  Every element is read once: L1 is passed by.
+template <int BYTES>
+__device__ __forceinline__ void fetch_units(uint32_t dst, const uint16_t* p) {
+#pragma unroll
+  for (int i = 0; i < 16; i += BYTES)
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst + i), "l"(p + i / 2), "n"(BYTES) : "memory");
+}
+
+// The walk's row to shared memory: cp.async in whole units, else plain loads, with zeros
+// past the row's end.  Units of 16 bytes are read once by one thread: L1 is passed by.
+// WIDE: every operand's unit is 16, so that the narrower ones are not asked for (they cost
+// an aligned act_grad 7 %).
+template <bool WIDE>
 __device__ __forceinline__ void fetch8(uint32_t dst, Walk& w, int c, int cols) {
-  if (w.unit) {
+  if (w.unit == 16) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(w.p) : "memory");
+  } else if (!WIDE && w.unit == 8) {
+    fetch_units<8>(dst, w.p);
+  } else if (!WIDE && w.unit == 4) {
+    fetch_units<4>(dst, w.p);
   } else {
     uint32_t q[4];
 #pragma unroll
@@ -62,24 +79,35 @@ __device__ __forceinline__ uint4 lds16(uint32_t addr) {
   return v;
 }
 
-template <int TYPE>
+template <int TYPE, bool WIDE>
 __device__ __forceinline__ void put8(const float (&v)[8], Walk& w, int c, int cols) {
-  storen<TYPE, 8>(v, const_cast<uint16_t*>(w.p), 0, c, cols, w.unit);
+  uint16_t* d = const_cast<uint16_t*>(w.p);
+  if (w.unit == 16) {
+    *reinterpret_cast<uint4*>(d) = pack8<TYPE>(v);
+  } else if (!WIDE && w.unit >= 4) {   // 8 or 4 bytes: four words either way
+    const uint4 q = pack8<TYPE>(v);
+    uint32_t* d4 = reinterpret_cast<uint32_t*>(d);
+    d4[0] = q.x, d4[1] = q.y, d4[2] = q.z, d4[3] = q.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (c + i < cols) store1<TYPE>(d, i, v[i]);
+  }
   w.p += w.step;
 }
 
 // One or two operands' rows pass through f(row, words of the first, of the second) in
 // order, from `r` on in steps of `rows`; `ring` is the thread's 16 bytes of slot 0.
-template <int OPS, typename F>
+template <int THREADS, int OPS, bool WIDE, typename F>
 __device__ __forceinline__ void stream_rows(uint32_t ring, Walk a, Walk b, int r, int rows, int n, int c, int cols, F f) {
-  constexpr uint32_t kOp = kThreads * 16, kSlot = OPS * kOp, kRing = kDepth * kSlot;
+  constexpr uint32_t kOp = THREADS * 16, kSlot = OPS * kOp, kRing = kDepth * kSlot;
   static_assert((kRing & (kRing - 1)) == 0, "power of two");
   int next = r;
   uint32_t in = 0, out = 0;
   auto fetch = [&] {
     if (next < n) {
-      fetch8(ring + in, a, c, cols);
-      if constexpr (OPS == 2) fetch8(ring + in + kOp, b, c, cols);
+      fetch8<WIDE>(ring + in, a, c, cols);
+      if constexpr (OPS == 2) fetch8<WIDE>(ring + in + kOp, b, c, cols);
     }
     fetch_commit();
     next += rows;
@@ -94,9 +122,9 @@ __device__ __forceinline__ void stream_rows(uint32_t ring, Walk a, Walk b, int r
   }
 }
 
-template <int TYPE, bool RES>
-__global__ void __launch_bounds__(kThreads) dropout_kernel(const __grid_constant__ DropoutArgs p, int lx, bool vx, bool vr,
-                                                           bool vy) {
+template <int TYPE, bool RES, bool WIDE>
+__global__ void __launch_bounds__(kThreads) dropout_kernel(const __grid_constant__ DropoutArgs p, int lx, int vx, int vr,
+                                                           int vy) {
   __shared__ uint4 ring[kDepth * (RES ? 2 : 1) * kThreads];
   const int t = (int)threadIdx.x;
   const int g = (int)(blockIdx.x << lx) + (t & ((1 << lx) - 1)), c = 8 * g;
@@ -105,7 +133,7 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(const __grid_constant
   const uint64_t off = drop_offset(p.drop);
   const int rows = (int)gridDim.y * (kThreads >> lx), r = (int)blockIdx.y * (kThreads >> lx) + (t >> lx);
   Walk y = walk(p.Y, p.ldy, vy, r, rows, c, p.M);
-  stream_rows<RES ? 2 : 1>(smem_u32(ring + t), walk(p.X, p.ldx, vx, r, rows, c, p.M),
+  stream_rows<kThreads, RES ? 2 : 1, WIDE>(smem_u32(ring + t), walk(p.X, p.ldx, vx, r, rows, c, p.M),
                            walk(p.res, p.ldr, vr, r, rows, c, p.M), r, rows, p.N, c, p.M,
                            [&](int row, auto first, auto second) {
     const uint4 b = p.drop.on ? drop_bits(p.drop, off, row, g) : make_uint4(0, 0, 0, 0);
@@ -118,7 +146,7 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(const __grid_constant
 #pragma unroll
       for (int j = 0; j < 8; j += 2) split2(add2(pair2(v[j], v[j + 1]), pair2(w[j], w[j + 1])), v[j], v[j + 1]);
     }
-    put8<TYPE>(v, y, c, p.M);
+    put8<TYPE, WIDE>(v, y, c, p.M);
   });
   griddep_launch();
 }
@@ -126,12 +154,12 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(const __grid_constant
 // A cluster's CTAs share the rows of one slab of columns.  Each thread's eight column
 // sums meet the CTA's other rows in shared memory and the other CTAs' over distributed
 // shared memory, always in the same order.
-template <int TYPE, int ACT>
-__global__ void __launch_bounds__(kThreads, 4) act_grad_kernel(const __grid_constant__ ActGradArgs p, int lx, bool vy, bool vz,
-                                                               bool vd) {
-  __shared__ uint4 ring[kDepth * (ACT == kActNone ? 1 : 2) * kThreads];
+template <int TYPE, int ACT, int THREADS, bool WIDE>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) act_grad_kernel(const __grid_constant__ ActGradArgs p, int lx,
+                                                                           int vy, int vz, int vd) {
+  extern __shared__ uint4 ring[];                 // kDepth rows of one or two operands
   float* part = reinterpret_cast<float*>(ring);   // the sums, once the ring is drained
-  const int t = (int)threadIdx.x, ty = kThreads >> lx, tx = 1 << lx;
+  const int t = (int)threadIdx.x, ty = THREADS >> lx, tx = 1 << lx;
   const int S = (int)gridDim.y, rank = (int)blockIdx.y;   // the cluster is the grid's y
   const int g = (int)(blockIdx.x << lx) + (t & (tx - 1)), c = 8 * g;
   float sum[8] = {};
@@ -140,7 +168,7 @@ __global__ void __launch_bounds__(kThreads, 4) act_grad_kernel(const __grid_cons
     const uint64_t off = drop_offset(p.drop);
     const int rows = S * ty, r = rank * ty + (t >> lx);
     Walk d = walk(p.dZ, p.lddz, vd, r, rows, c, p.M);
-    stream_rows<ACT == kActNone ? 1 : 2>(smem_u32(ring + t), walk(p.dY, p.lddy, vy, r, rows, c, p.M),
+    stream_rows<THREADS, ACT == kActNone ? 1 : 2, WIDE>(smem_u32(ring + t), walk(p.dY, p.lddy, vy, r, rows, c, p.M),
                                          walk(p.Z, p.ldz, vz, r, rows, c, p.M), r, rows, p.N, c, p.M,
                                          [&](int row, auto first, auto second) {
       const uint4 b = p.drop.on ? drop_bits(p.drop, off, row, g) : make_uint4(0, 0, 0, 0);
@@ -154,7 +182,7 @@ __global__ void __launch_bounds__(kThreads, 4) act_grad_kernel(const __grid_cons
           split2(mul2(pair2(v[j], v[j + 1]), act_slope2<ACT>(pair2(w[j], w[j + 1]))), v[j], v[j + 1]);
       }
       if (p.drop.on) drop8(v, p.drop, b);
-      if (p.dZ) put8<TYPE>(v, d, c, p.M);
+      if (p.dZ) put8<TYPE, WIDE>(v, d, c, p.M);
 #pragma unroll
       for (int j = 0; j < 8; j += 2)
         split2(add2(pair2(sum[j], sum[j + 1]), pair2(v[j], v[j + 1])), sum[j], sum[j + 1]);
@@ -166,19 +194,24 @@ __global__ void __launch_bounds__(kThreads, 4) act_grad_kernel(const __grid_cons
 #pragma unroll
   for (int j = 0; j < 8; ++j) part[threadIdx.x * 8 + j] = sum[j];
   __syncthreads();
-  // column i of the slab: thread i adds the rows' sums up
-  const int cols = 8 * tx;
+  // the rows' sums of one column are added by THREADS / cols threads, then theirs by one
+  const int cols = 8 * tx, segs = THREADS >> (lx + 3), i = t & (cols - 1);
   float s = 0.f;
-  if ((int)threadIdx.x < cols)
-    for (int k = 0; k < ty; ++k) s += part[k * cols + (int)threadIdx.x];
+  for (int k = t >> (lx + 3); k < ty; k += segs) s += part[k * cols + i];
   __syncthreads();
-  if ((int)threadIdx.x < cols) part[threadIdx.x] = s;
+  part[t] = s;
+  __syncthreads();
+  s = 0.f;
+  if (t < cols)
+    for (int k = 0; k < segs; ++k) s += part[k * cols + t];
+  __syncthreads();
+  if (t < cols) part[t] = s;
   cluster_sync();
-  const int col = (int)(blockIdx.x << lx) * 8 + (int)threadIdx.x;
-  if (rank == 0 && (int)threadIdx.x < cols && col < p.M) {
-    float t = 0.f;
-    for (int k = 0; k < S; ++k) t += __uint_as_float(ld_dsmem_u32(mapa_shared(&part[threadIdx.x], (uint32_t)k)));
-    p.dbias[col] = t;
+  const int col = (int)blockIdx.x * cols + t;
+  if (rank == 0 && t < cols && col < p.M) {
+    float sum_all = 0.f;
+    for (int k = 0; k < S; ++k) sum_all += __uint_as_float(ld_dsmem_u32(mapa_shared(&part[t], (uint32_t)k)));
+    p.dbias[col] = sum_all;
   }
   cluster_sync_relaxed();   // no CTA leaves while its sums are read
 }
@@ -189,61 +222,105 @@ int log2_up(int n, int most) {
   return l;
 }
 
-template <int TYPE, int ACT>
-cudaError_t launch_act_grad_typed(const ActGradArgs& a) {
-  const int groups = (a.M + 7) / 8;
-  // Columns per CTA (16 to 128) and CTAs per cluster.  What counts, measured over all
-  // pairs at nine shapes: SMs with equal numbers of CTAs, three or four each (2048 x 11008
-  // with dropout: 35.2 us with 86 slabs x 8 = 4.65 per SM, 41.6 us with 86 x 4 = 2.3),
-  // four rows per thread (300 x 11008: 7.3 us with 86 x 4, 9.3 us with 86 x 8) and rows
-  // of whole 128-byte lines (8192 x 1024: 17 us with 32 slabs x 8, 20 us with 64 x 8);
-  // clusters of 16 pay for narrow matrices alone (16384 x 64: 7.8 against 12 us), and
-  // sizes between the powers of two do not (172 x 6: 38.2 us).
+// How a call is cut: 2^lx column groups per CTA, S CTAs (a cluster where there are sums)
+// on the rows of a slab, threads per CTA.
+struct GradPlan {
+  int lx, S, threads;
+};
+
+// What counts, measured over all pairs of slab width and S at twelve shapes: SMs with equal
+// numbers of CTAs, three or four of 256 threads each (2048 x 11008 with dropout: 34.5 us
+// with 86 slabs x 8, 41.7 us with 86 x 4), four rows per thread (300 x 11008: 7.5 us with
+// 86 x 4, 9.0 us with 86 x 8) and rows of whole 128-byte lines (2048 x 4096: 15.6 us with
+// 64 slabs x 8, 18.3 us with 128 x 8).  Sizes of S between the powers of two never paid
+// (2048 x 11008: 38.2 us with 172 x 6), clusters of 16 for narrow matrices alone (16384 x
+// 64: 7.5 against 11.7 us).  CTAs of 1024 threads fill the SMs where few slabs with at most
+// 8 CTAs on each would not (8192 x 1024: 16.0 against 19.7 us, 32768 x 512 without an
+// activation: 18.1 against 31.2 us).
+GradPlan grad_plan(const ActGradArgs& a) {
+  // CTAs of clusters of 1, 2, 4, 8, 16 that are resident at once on 148 SMs
+  static const long kRoom[2][5] = {{740, 740, 740, 740, 496}, {148, 148, 132, 120, 112}};
   static const double kLines[5] = {0, 0.6, 0.9, 0.98, 1.0};
-  int lx = log2_up(groups, 4), S = 1;
-  double best = 0;
-  for (int l = std::min(lx, 4); l >= std::min(lx, 1); --l) {
-    const long slabs = (groups + (1 << l) - 1) >> l, sms = a.num_sms;
-    const int ty = kThreads >> l;
-    const int most = slabs * 8 <= sms / 2 ? 16 : 8;
-    for (int k = 1; k <= most && (k == 1 || k / 2 * ty < a.N); k *= 2) {
-      const long ctas = slabs * k;
-      const double even = (double)ctas / ((ctas + sms - 1) / sms * sms);
-      const double fill = std::min(1.0, ctas / (3.5 * sms)), depth = std::min(1.0, a.N / (4.0 * ty * k));
-      const double score = even * std::sqrt(fill * depth) * kLines[std::max(l, 1)] * groups / (slabs << l);
-      if (score > best * 1.005) best = score, lx = l, S = k;
-    }
+  const int groups = (a.M + 7) / 8, most_lx = std::min(log2_up(groups, 4), 4);
+  GradPlan best = {most_lx, 1, kThreads};
+  if (!a.dbias) {   // rows go to any number of CTAs
+    const long slabs = (groups + (1 << most_lx) - 1) >> most_lx, ty = kThreads >> most_lx;
+    best.S = (int)std::min({((long)a.N + ty - 1) / ty, std::max(1L, 5L * a.num_sms / slabs), 65535L});
+    return best;
   }
+  double top = 0;
+  for (int threads = kThreads; threads <= 1024; threads *= 4)
+    for (int l = most_lx; l >= std::min(most_lx, 1); --l) {
+      const long slabs = (groups + (1 << l) - 1) >> l, sms = a.num_sms;
+      const int ty = threads >> l, most = slabs * 8 <= sms / 2 && threads == kThreads ? 16 : 8;
+      for (int k = 1; k <= most && (k == 1 || k / 2 * ty < a.N); k *= 2) {
+        const long ctas = slabs * k, room = kRoom[threads > kThreads][log2_up(k, 4)];
+        const double even = ctas <= room ? (double)ctas / ((ctas + sms - 1) / sms * sms)
+                                         : (double)ctas / ((ctas + room - 1) / room * (threads > kThreads ? sms : 5 * sms));
+        const double fill = std::min(1.0, ctas * (threads / kThreads) / (3.5 * sms));
+        const double depth = std::min(1.0, a.N / (4.0 * ty * k));
+        const double score = even * std::sqrt(fill * depth) * kLines[std::max(l, 1)] * groups / (slabs << l) *
+                             (threads == kThreads ? 1.0 : 0.9);
+        if (score > top * 1.005) top = score, best = {l, k, threads};
+      }
+    }
+  return best;
+}
+
+template <int TYPE, int ACT, int THREADS, bool WIDE>
+cudaError_t launch_act_grad_typed(const ActGradArgs& a, const GradPlan& pl) {
+  auto kernel = act_grad_kernel<TYPE, ACT, THREADS, WIDE>;
+  constexpr int smem = kDepth * (ACT == kActNone ? 1 : 2) * THREADS * 16;   // at least the sums' 32 bytes a thread
+  static_assert(smem >= THREADS * 32, "sums");
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 1;
-  attr[0].val.clusterDim.y = S;
-  attr[0].val.clusterDim.z = 1;
-  cfg.gridDim = dim3((groups + (1 << lx) - 1) >> lx, S);
-  cfg.blockDim = dim3(kThreads);
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 1;
+  attr[1].val.clusterDim.y = pl.S;
+  attr[1].val.clusterDim.z = 1;
+  cfg.gridDim = dim3(((a.M + 7) / 8 + (1 << pl.lx) - 1) >> pl.lx, pl.S);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = a.stream;
   cfg.attrs = attr;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.numAttrs = 2;
-  if (S > 8) {   // clusters above the portable size
-    const cudaError_t e = cudaFuncSetAttribute(act_grad_kernel<TYPE, ACT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return e;
-  }
-  return cudaLaunchKernelEx(&cfg, act_grad_kernel<TYPE, ACT>, a, lx, vec_rows(a.dY, a.lddy), vec_rows(a.Z, a.ldz),
-                            vec_rows(a.dZ, a.lddz));
+  cfg.numAttrs = a.dbias ? 2 : 1;
+  cudaError_t e = cudaSuccess;
+  if (smem > 48 * 1024) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess && a.dbias && pl.S > 8)   // clusters above the portable size
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e != cudaSuccess) return e;
+  return cudaLaunchKernelEx(&cfg, kernel, a, pl.lx, row_unit(a.dY, a.lddy), row_unit(a.Z, a.ldz),
+                            row_unit(a.dZ, a.lddz));
+}
+
+template <int TYPE, int ACT>
+cudaError_t launch_act_grad_sized(const ActGradArgs& a) {
+  const GradPlan pl = grad_plan(a);
+  const bool wide = row_unit(a.dY, a.lddy) == 16 && (ACT == kActNone || row_unit(a.Z, a.ldz) == 16) &&
+                    (!a.dZ || row_unit(a.dZ, a.lddz) == 16);
+  if (pl.threads == 1024)
+    return wide ? launch_act_grad_typed<TYPE, ACT, 1024, true>(a, pl) : launch_act_grad_typed<TYPE, ACT, 1024, false>(a, pl);
+  return wide ? launch_act_grad_typed<TYPE, ACT, kThreads, true>(a, pl)
+              : launch_act_grad_typed<TYPE, ACT, kThreads, false>(a, pl);
 }
 
 template <int TYPE>
 cudaError_t launch_act_grad_act(const ActGradArgs& a) {
   switch (a.act) {
-    case kActRelu: return launch_act_grad_typed<TYPE, kActRelu>(a);
-    case kActGelu: return launch_act_grad_typed<TYPE, kActGelu>(a);
-    case kActGeluTanh: return launch_act_grad_typed<TYPE, kActGeluTanh>(a);
-    case kActSilu: return launch_act_grad_typed<TYPE, kActSilu>(a);
-    default: return launch_act_grad_typed<TYPE, kActNone>(a);
+    case kActRelu: return launch_act_grad_sized<TYPE, kActRelu>(a);
+    case kActGelu: return launch_act_grad_sized<TYPE, kActGelu>(a);
+    case kActGeluTanh: return launch_act_grad_sized<TYPE, kActGeluTanh>(a);
+    case kActSilu: return launch_act_grad_sized<TYPE, kActSilu>(a);
+    default: return launch_act_grad_sized<TYPE, kActNone>(a);
   }
+}
+
+template <int TYPE>
+auto dropout_pick(bool res, bool wide) {
+  return res ? (wide ? dropout_kernel<TYPE, true, true> : dropout_kernel<TYPE, true, false>)
+             : (wide ? dropout_kernel<TYPE, false, true> : dropout_kernel<TYPE, false, false>);
 }
 
 }  // namespace
@@ -255,7 +332,7 @@ cudaError_t launch_dropout(const DropoutArgs& a) {
   const long slabs = (groups + (1 << lx) - 1) >> lx;
   const long most = std::max(1L, 6L * a.num_sms / slabs);
   const dim3 grid((unsigned)slabs, (unsigned)std::min({((long)a.N + ty - 1) / ty, most, 65535L}));
-  const bool vx = vec_rows(a.X, a.ldx), vr = vec_rows(a.res, a.ldr), vy = vec_rows(a.Y, a.ldy);
+  const int vx = row_unit(a.X, a.ldx), vr = row_unit(a.res, a.ldr), vy = row_unit(a.Y, a.ldy);
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -265,8 +342,9 @@ cudaError_t launch_dropout(const DropoutArgs& a) {
   cfg.stream = a.stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  auto kernel = a.type == kTypeF16 ? (a.res ? dropout_kernel<kTypeF16, true> : dropout_kernel<kTypeF16, false>)
-                                   : (a.res ? dropout_kernel<kTypeBF16, true> : dropout_kernel<kTypeBF16, false>);
+  const bool wide = vx == 16 && vy == 16 && (!a.res || vr == 16);
+  auto kernel = dropout_pick<kTypeBF16>(a.res, wide);
+  if (a.type == kTypeF16) kernel = dropout_pick<kTypeF16>(a.res, wide);
   return cudaLaunchKernelEx(&cfg, kernel, a, lx, vx, vr, vy);
 }
 

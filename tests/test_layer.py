@@ -413,7 +413,8 @@ def act_grad_ref(dy, z, act, p, seed, offset):
 @pytest.mark.gpu
 @pytest.mark.parametrize("act", ACT_NAMES)
 @pytest.mark.parametrize("type", ["f16", "bf16"])
-@pytest.mark.parametrize("size", [(1, 1), (1, 8), (3, 67), (37, 1003), (64, 64), (300, 520), (2500, 136)], ids=str)
+@pytest.mark.parametrize("size", [(1, 1), (1, 8), (3, 67), (37, 1003), (64, 64), (300, 520), (2500, 136), (5000, 300), (9000, 1024), (4500, 514)],
+                         ids=str)
 def test_act_grad(gemm, size, type, act):
     N, M = size
     t = ttype(type)
@@ -446,7 +447,7 @@ def test_act_grad_strided_and_limits(gemm):
     N, M, t = 70, 200, torch.float16
     dy0, z0 = rand((N, M), t, 1), rand((N, M), t, 2)
     z0[3, 5], z0[4, 6], z0[5, 7] = float("inf"), float("-inf"), float("nan")
-    for pad, shift in ((8, 8), (5, 3)):
+    for pad, shift in ((8, 8), (4, 4), (2, 2), (5, 3)):
         dy, z = put(dy0, M + pad, shift), put(z0, M + pad, shift)
         for act in ("relu", "gelu", "gelu_tanh", "silu"):
             buf, dz = strided((N, M), t, M + pad, shift, 7.0)
@@ -496,7 +497,7 @@ def test_dropout_strided(gemm):
     x0, r0 = rand((N, M), t, 1), rand((N, M), t, 2)
     f = torch.from_numpy(factors(N, M, 0.3, 1, 2)).cuda()
     ref = x0.double() * f + r0.double()
-    for pad, shift in ((8, 8), (8, 4), (3, 1)):
+    for pad, shift in ((8, 8), (8, 4), (4, 8), (2, 4), (6, 2), (3, 1)):
         buf, y = strided((N, M), t, M + pad, shift, 7.0)
         G.dropout(0, G.TYPES["bf16"], put(x0, M + pad, shift), y, N, M, 0.3, 1, 2, residual=put(r0, M + pad, shift),
                   ldx=M + pad, ldr=M + pad, ldy=M + pad, stream=stream())
