@@ -122,6 +122,8 @@ __device__ __forceinline__ void stream_rows(uint32_t ring, Walk a, Walk b, int r
   }
 }
 
+// Bound by HBM: 4096 x 4096 bf16 with a residual 18.6 us, 5.4 TB/s (17.1 us without
+// dropout); 33 x 4104 1.4 us.
 template <int TYPE, bool RES, bool WIDE>
 __global__ void __launch_bounds__(kThreads) dropout_kernel(const __grid_constant__ DropoutArgs p, int lx, int vx, int vr,
                                                            int vy) {
@@ -154,6 +156,9 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(const __grid_constant
 // A cluster's CTAs share the rows of one slab of columns.  Each thread's eight column
 // sums meet the CTA's other rows in shared memory and the other CTAs' over distributed
 // shared memory, always in the same order.
+// 2048 x 11008 bf16 with the sums: 19.2 us without an activation (4.7 TB/s), 29 us with
+// gelu (4.6 TB/s), 35 us with gelu and dropout, where the 36 instructions per element fill
+// 58 % of all issue slots.
 template <int TYPE, int ACT, int THREADS, bool WIDE>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) act_grad_kernel(const __grid_constant__ ActGradArgs p, int lx,
                                                                            int vy, int vz, int vd) {

@@ -30,6 +30,7 @@ constexpr int kKb = 64;            // contraction elements per stage: one 128-by
 constexpr int kBoxBytes = 64 * 128;   // one MN-major box: 64 contraction rows x 64 elements
 constexpr int kSmemMax = 232448;
 constexpr int kMaxSplit = 8;       // portable cluster size
+constexpr int kSegment = 8;        // f32 results: stages per partial sum (linear_pair.cu says why)
 
 struct EpiArgs {
   const void *bias, *res;
@@ -98,8 +99,9 @@ inline EpiArgs epilogue(const LinearArgs& a) {
   e.depth = a.depth;
   e.drop = a.drop;
   e.bias_vec = aligned16(a.bias);
-  e.out_vec = aligned16(a.out) && a.ldo % 8 == 0;
-  e.res_vec = aligned16(a.res) && a.ldr % 8 == 0;
+  const int es = a.out_type == kTypeF32 ? 4 : 2;
+  e.out_vec = aligned16(a.out) && a.ldo * es % 16 == 0;
+  e.res_vec = aligned16(a.res) && a.ldr * es % 16 == 0;
   e.pre_vec = aligned16(a.pre) && a.ldz % 8 == 0;
   e.dev_err = a.dev_err;
   return e;
@@ -133,7 +135,11 @@ cudaError_t prepare(Once& once, Kernel k, int smem, cudaLaunchConfig_t& cfg, int
 // rows_op, cols_op: the stored operands whose rows or columns index the result's rows
 // and columns (A and B of LinearArgs, packed where they had to be)
 cudaError_t launch_pair(const LinearArgs& a, const Operand& rows_op, const Operand& cols_op);
-// bn rows per CTA (16, 32, 64, 128, 256; dW from 64), clusters of `split`
+// f32 results: the contraction that one CTA of the split kernel takes, in partial sums that
+// fit its share of TMEM
+constexpr int split_segments(int bn) { return bn == 256 ? 2 : 256 / bn; }
+// bn rows per CTA (16, 32, 64, 128, 256; dW from 64), clusters of `split`; f32 results: at most
+// kSegment * split_segments(bn) blocks of the contraction per CTA
 cudaError_t launch_split(const LinearArgs& a, const Operand& rows_op, const Operand& cols_op, int bn, int split);
 
 }  // namespace mlpg

@@ -21,11 +21,15 @@ namespace {
 // (measured against 64 bits: 6e-7 after 512, 5e-6 after 4096).  So every 512 deep the
 // partial sum leaves TMEM and is added in registers, rounded to nearest.  16-bit results,
 // whose own rounding is 2^-12 or 2^-9, keep one accumulation.
+//
+// Bound by the tensor cores, and over a run of such calls by the board's power: linear
+// 2048 x 4096 x 11008 bf16 147 us, 1250 TFLOP/s (76 % of the measured burst, 90 % of the
+// sustained rate), with gelu_tanh, bias and Z 151 us; dw 2048 x 4096 x 11008 147 us, in f32
+// 167 us.
 constexpr int kPairThreads = 640;
 constexpr int kEpiWarps = 16;
 constexpr int kEpiBuf = 4096;      // a warp's staging: 32 rows x 128 bytes
 constexpr int kGroupRows = 8;      // row tiles per group of the tile order
-constexpr int kSegment = 8;        // F32: stages per partial sum
 
 template <int OP>
 struct PairCfg {

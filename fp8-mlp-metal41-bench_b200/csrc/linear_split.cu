@@ -13,9 +13,17 @@ namespace {
 // sums into their own shared memory, and each then sums and finishes its share of the
 // tile over distributed shared memory, in rank order: no workspace, no atomics, the
 // same result every time.
+//
+// Bound by HBM while the weights are read once: 1 x 4096 x 11008 bf16 16.3 us, 5.5 TB/s of
+// weights with the launch and the sums in it; 13 x 11008 x 4096 17.5 us.  From 64 rows on by
+// what an SM reads from L2 (about 100 GB/s): 256 x 4096 x 4096 15.4 us.
+//
+// f32 results (dW): the contraction is cut into partial sums of kSegment blocks here too,
+// side by side in TMEM and added with rounding when they are read out (8192 x 1024 x 1024:
+// 32.6 us, the pair kernel 47 us).
 constexpr int kSplitThreads = 256;
 
-template <int OP, int BN>
+template <int OP, int BN, bool F32>
 struct SplitCfg {
   static constexpr bool C_MN = OP != kOpDx, R_MN = OP == kOpDw;
   static constexpr int C_BYTES = 128 * 128, R_BYTES = BN * 128;
@@ -26,7 +34,8 @@ struct SplitCfg {
   static constexpr int PER_SM = BN <= 128 ? 2 : 1;
   static constexpr int BAR_OFF = STAGES * STAGE_BYTES;
   static constexpr int SMEM = BAR_OFF + 512 + 1024;
-  static constexpr uint32_t TMEM_COLS = BN < 32 ? 32 : BN;
+  static constexpr int SEGS = F32 ? split_segments(BN) : 1;   // accumulators, kSegment blocks each
+  static constexpr uint32_t TMEM_COLS = BN < 32 ? 32 : SEGS * BN;
   static constexpr uint32_t IDESC = (1u << 4) | ((C_MN ? 1u : 0u) << 15) | ((R_MN ? 1u : 0u) << 16) |
                                     ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
   static_assert(BN * 512 <= BAR_OFF, "partial sums fit the ring");
@@ -65,11 +74,11 @@ __device__ __forceinline__ uint32_t cluster_nctarank() {
   return r;
 }
 
-template <int OP, int TYPE, int BN>
-__global__ void __launch_bounds__(kSplitThreads, SplitCfg<OP, BN>::PER_SM)
+template <int OP, int TYPE, int BN, bool F32>
+__global__ void __launch_bounds__(kSplitThreads, SplitCfg<OP, BN, F32>::PER_SM)
     linear_split_kernel(const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmR,
                         const __grid_constant__ EpiArgs p) {
-  using C = SplitCfg<OP, BN>;
+  using C = SplitCfg<OP, BN, F32>;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -133,10 +142,13 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<OP, BN>::PER_SM)
       if (!mbar_wait(&bars->full[stage], phase, ctl, 0x300 + stage)) { aborted_any = true; break; }
       tc_fence_after();
       const uint32_t a = smem_base + stage * C::STAGE_BYTES, b = a + C::C_BYTES;
+      const int run = kb - kb0;   // f32: a fresh accumulator every kSegment blocks
+      const uint32_t d = F32 ? tmem_base + (uint32_t)(run / kSegment * BN) : tmem_base;
+      const bool fresh = F32 ? run % kSegment == 0 : run == 0;
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk)
-        tc_mma<kKindF16>(tmem_base, op_desc(a, C::C_MN, kk), op_desc(b, C::R_MN, kk), idesc,
-                         (kb != kb0 || kk != 0) ? 1u : 0u);
+        tc_mma<kKindF16>(d, op_desc(a, C::C_MN, kk), op_desc(b, C::R_MN, kk), idesc,
+                         (!fresh || kk != 0) ? 1u : 0u);
       tc_commit(&bars->empty[stage]);
       if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
     }
@@ -156,6 +168,16 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<OP, BN>::PER_SM)
         if constexpr (CH == 16) tmem_ld_32x32b_x16(acc + (uint32_t)n0, r);
         else tmem_ld_32x32b_x32(acc + (uint32_t)n0, r);
         tmem_ld_wait();
+        if constexpr (F32) {   // the other partial sums, added with rounding
+#pragma unroll 1
+          for (int g = 1; g * kSegment < kb1 - kb0; ++g) {
+            uint32_t x[CH];
+            tmem_ld_32x32b_x32(acc + (uint32_t)(g * BN + n0), x);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < CH; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) + __uint_as_float(x[i]));
+          }
+        }
 #pragma unroll
         for (int i = 0; i < CH; ++i)
           if (n0 + i < nrows) part[(n0 + i) * 128 + q * 32 + lane] = __uint_as_float(r[i]);
@@ -211,13 +233,39 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<OP, BN>::PER_SM)
         act_fwd_n(v, p.act);
         if (p.drop.on) drop4(v, p.drop, off, row, c);
       }
-      if (p.res) {
-        float r[4];
-        loadn<TYPE, 4>(r, p.res, (size_t)row * p.ldr + c, c, p.cols, p.res_vec);
+      const size_t oa = (size_t)row * p.ldo + c, ra = (size_t)row * p.ldr + c;
+      if constexpr (F32) {
+        float* out = static_cast<float*>(p.out) + oa;
+        const float* res = static_cast<const float*>(p.res) + ra;
+        if (p.res) {
+          float r[4] = {};
+          if (p.res_vec && c + 4 <= p.cols) {
+            const float4 q = *reinterpret_cast<const float4*>(res);
+            r[0] = q.x, r[1] = q.y, r[2] = q.z, r[3] = q.w;
+          } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] += r[j];
+            for (int j = 0; j < 4; ++j)
+              if (c + j < p.cols) r[j] = res[j];
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] += r[j];
+        }
+        if (p.out_vec && c + 4 <= p.cols) {
+          *reinterpret_cast<float4*>(out) = make_float4(v[0], v[1], v[2], v[3]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (c + j < p.cols) out[j] = v[j];
+        }
+      } else {
+        if (p.res) {
+          float r[4];
+          loadn<TYPE, 4>(r, p.res, ra, c, p.cols, p.res_vec);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] += r[j];
+        }
+        storen<TYPE, 4>(v, p.out, oa, c, p.cols, p.out_vec);
       }
-      storen<TYPE, 4>(v, p.out, (size_t)row * p.ldo + c, c, p.cols, p.out_vec);
     }
   }
   // no CTA leaves while another reads its partial sums; nothing is handed over, so the
@@ -226,9 +274,9 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<OP, BN>::PER_SM)
   if (S > 1) cluster_sync_relaxed();
 }
 
-template <int OP, int TYPE, int BN>
+template <int OP, int TYPE, int BN, bool F32 = false>
 cudaError_t launch_one(const LinearArgs& a, const Operand& x, const Operand& y, int S) {
-  using C = SplitCfg<OP, BN>;
+  using C = SplitCfg<OP, BN, F32>;
   const EpiArgs p = epilogue(a);
   CUtensorMap tmC, tmR;
   if (!map_rows(&tmC, y.p, y.ld, y.rows, y.cols, 2, C::C_MN ? kKb : 128) ||
@@ -249,7 +297,7 @@ cudaError_t launch_one(const LinearArgs& a, const Operand& x, const Operand& y, 
   cfg.attrs = attr;
   cfg.numAttrs = 2;
   static Once once;
-  auto k = linear_split_kernel<OP, TYPE, BN>;
+  auto k = linear_split_kernel<OP, TYPE, BN, F32>;
   cudaError_t e = prepare(once, k, C::SMEM, cfg, nullptr);
   if (e != cudaSuccess) return e;
   return cudaLaunchKernelEx(&cfg, k, tmC, tmR, p);
@@ -260,6 +308,13 @@ cudaError_t launch_bn(const LinearArgs& a, const Operand& x, const Operand& y, i
   if constexpr (OP != kOpDw) {
     if (bn == 16) return launch_one<OP, TYPE, 16>(a, x, y, S);
     if (bn == 32) return launch_one<OP, TYPE, 32>(a, x, y, S);
+  }
+  if constexpr (OP == kOpDw) {
+    if (a.out_type == kTypeF32) {
+      if (bn == 64) return launch_one<OP, TYPE, 64, true>(a, x, y, S);
+      if (bn == 128) return launch_one<OP, TYPE, 128, true>(a, x, y, S);
+      return launch_one<OP, TYPE, 256, true>(a, x, y, S);
+    }
   }
   if (bn == 64) return launch_one<OP, TYPE, 64>(a, x, y, S);
   if (bn == 128) return launch_one<OP, TYPE, 128>(a, x, y, S);

@@ -388,13 +388,14 @@ def test_gradient_products_strided(gemm, size, pad, shift):
 def test_dw_long_sum_in_32_bits(gemm):
     # accumulated over many rows, the f32 gradient stays within 1e-6 of the 64-bit sum (2-norm): partial sums of
     # 512 rows leave the tensor cores, whose adds cut, before 512/16 of them have lost 32 * 2^-25 = 1e-6
-    N, K, M = 8192, 264, 512
-    x, dz = rand((N, K), torch.bfloat16, 1), rand((N, M), torch.bfloat16, 2)
-    dw = torch.empty(K, M, device="cuda")
-    G.linear_dw(0, G.TYPES["bf16"], x, dz, dw, N, K, M, out_type=G.TYPES["f32"], stream=stream())
-    G.sync(0, stream())
-    ref = x.double().t() @ dz.double()
-    assert float((dw.double() - ref).norm() / ref.norm()) <= 1e-6
+    for N, K, M in ((700, 264, 512), (4000, 264, 512), (8192, 264, 512), (16384, 64, 136), (30000, 264, 512),
+                    (3000, 1032, 520), (2000, 2056, 4104), (9000, 2056, 72)):
+        x, dz = rand((N, K), torch.bfloat16, 1), rand((N, M), torch.bfloat16, 2)
+        dw = torch.empty(K, M, device="cuda")
+        G.linear_dw(0, G.TYPES["bf16"], x, dz, dw, N, K, M, out_type=G.TYPES["f32"], stream=stream())
+        G.sync(0, stream())
+        ref = x.double().t() @ dz.double()
+        assert float((dw.double() - ref).norm() / ref.norm()) <= 1e-6, (N, K, M)
 
 
 # ---- the epilogue's gradient ----------------------------------------------------------------
