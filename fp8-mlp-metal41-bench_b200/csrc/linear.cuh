@@ -36,7 +36,7 @@ struct EpiArgs {
   const void *bias, *res;
   void *out, *pre;
   long ldo, ldr, ldz;
-  int type, out_type, act;
+  int act;
   int rows, cols, depth;
   DropArgs drop;
   bool bias_vec, out_vec, res_vec, pre_vec;   // 16-byte aligned base and rows
@@ -91,8 +91,6 @@ inline EpiArgs epilogue(const LinearArgs& a) {
   e.ldo = a.ldo;
   e.ldr = a.ldr;
   e.ldz = a.ldz;
-  e.type = a.type;
-  e.out_type = a.out_type;
   e.act = a.act;
   e.rows = a.rows;
   e.cols = a.cols;
