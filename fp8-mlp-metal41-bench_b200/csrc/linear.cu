@@ -57,32 +57,43 @@ struct Plan {
 constexpr int kRoom[2][kMaxSplit] = {{148, 148, 135, 132, 130, 132, 105, 120}, {296, 296, 279, 284, 280, 270, 259, 264}};
 
 // An estimate of the split kernel's time in us in a stream of such calls: loads bound by the
-// busiest SM (102 GB/s, 77 where a single CTA of a kind that shares its SM keeps but half
-// of the bytes in flight, 0.6 us per block at 256 rows) or by HBM (6.6 TB/s, less with
-// fewer CTAs than SMs), then the sums over the cluster and the epilogue.  The constants are
-// a fit to 99 products of 1 .. 4096 rows, every bn and cluster size timed: the choice is on
-// average 1.4 % slower than the best of them and at most 21 %.
+// busiest SM (102 GB/s, 76 where a single CTA of a kind that shares its SM keeps but half
+// of the bytes in flight, 0.59 us per block at 256 rows) or by HBM (6.6 TB/s, less with
+// fewer CTAs than SMs), or a little longer than either where both are near; then the sums
+// over the cluster and the epilogue.  Clusters of more than four cost extra (128 x 4096 x
+// 4096 in parts of 128 rows: 13.1 us with four CTAs, 14.0 with eight and half the loads
+// each): eight CTAs of one GPC have to be free at once.  The constants are a fit to 156
+// products of 1 .. 4096 rows, every bn and cluster size timed: the choice is on average 0.7 %
+// slower than the best of them and at most 15 %.
 double split_time(const LinearArgs& a, int bn, int S) {
   const int per_sm = bn <= 128 ? 2 : 1, room = kRoom[per_sm - 1][S - 1];
   const long num_kb = (a.depth + kKb - 1) / kKb, kb = (num_kb + S - 1) / S;
   const long ctas = (long)((a.rows + bn - 1) / bn) * ((a.cols + 127) / 128) * S;
   const double on_sm = (double)((ctas * per_sm + room - 1) / room), rounds = (double)((ctas + room - 1) / room);
+  // the busiest SM ends a little faster where the others have less
+  const double share = on_sm < 2 ? 1 : 0.713 * on_sm + 0.287 * std::max(1.0, (double)(ctas * per_sm) / room);
   const double mb = (128 + bn) * 128e-6;   // a block of both operands
-  const double block = std::max(mb / (on_sm == 1 && per_sm == 2 ? 0.0772 : 0.1021), bn * 0.00238);
-  const double hbm = ((double)a.rows + a.cols) * num_kb * kKb * 2e-6 / 6.6 * (1 + 0.496 * std::max(0.0, 1 - ctas / 160.0));
+  const double load = share * kb * std::max(mb / (on_sm < 2 && per_sm == 2 ? 0.0755 : 0.102), bn * 0.0023);
+  const double hbm = ((double)a.rows + a.cols) * num_kb * kKb * 2e-6 / 6.6 * (1 + 0.54 * std::max(0.0, 1 - ctas / 160.0));
+  const double most = std::max(load, hbm);
+  double near = std::min(load, hbm) / most;
+  near *= near, near *= near, near *= near;
   const double n = std::min(bn, a.rows);
   static constexpr double kPow57[9] = {0, 1, 1.485, 1.871, 2.204, 2.503, 2.777, 3.032, 3.272};   // on_sm ^ 0.57
-  const double sums = S > 1 ? (0.267 + n * 0.0154 * (S - 1) / S) * kPow57[std::min((int)on_sm, 8)] : 0;
-  return 2.54 + std::max(on_sm * kb * block, hbm) + sums + n / S * 0.0152 * on_sm + n * 0.0053 + (rounds - 1) * 3.13;
+  double sums = S > 1 ? 0.248 + n * 0.016 * (S - 1) / S : 0;
+  if (S > 4) sums += (0.108 + n * 0.0017) * (S - 4);
+  return 2.41 + most * (1 + 0.13 * near) + sums * kPow57[std::min((int)on_sm, 8)] + n / S * 0.0151 * on_sm +
+         n * 0.0043 + (rounds - 1) * 2.54;
 }
 
-// The same for the pair kernel: rounds of tiles over the pairs, or HBM.
+// The same for the pair kernel: rounds of tiles over the pairs, or HBM (few rounds hide
+// little of a cold start: 3.35 TB/s).
 double pair_time(const LinearArgs& a) {
   const long num_kb = (a.depth + kKb - 1) / kKb;
   const long tiles = (long)((a.rows + 255) / 256) * ((a.cols + 255) / 256), pairs = a.num_sms / 2;
   const double rounds = (double)((tiles + pairs - 1) / pairs);
-  const double hbm = ((double)a.rows + a.cols) * num_kb * kKb * 2e-6 / 6.3 + (double)a.rows * a.cols * 2e-6 / 5.0;
-  return 2.77 + std::max(rounds * std::max(num_kb * 0.337, 1.19) + 3.79, hbm);
+  const double hbm = ((double)a.rows + a.cols) * num_kb * kKb * 2e-6 / 3.35 + (double)a.rows * a.cols * 2e-6 / 5.0;
+  return 2.85 + std::max(rounds * std::max(num_kb * 0.392, 0.38) + 2.59, hbm);
 }
 
 Plan plan(const LinearArgs& a) {
