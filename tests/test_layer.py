@@ -385,6 +385,28 @@ def test_gradient_products_strided(gemm, size, pad, shift):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("size,pad", [((333, 1032, 2056), 0), ((70, 2056, 1804), 8), ((600, 2100, 2058), 6),
+                                      ((1, 4096, 520), 0), ((1100, 3000, 1300), 4), ((65, 1, 9000), 0)], ids=str)
+def test_dw_in_place_equals_dw_beside(gemm, size, pad):
+    # one addition of the same two numbers, rounded to nearest, wherever the old value comes from: the same bits
+    N, K, M = size
+    x, dz, r = rand((N, K), torch.bfloat16, 1), rand((N, M), torch.bfloat16, 2), rand((K, M), torch.float32, 3)
+    r[0, 5], r[K // 2, 7], r[K - 1, M - 1] = float("inf"), float("nan"), 3e38
+    buf, dw = strided((K, M), torch.float32, M + pad, 0, 7.0)
+    dw.copy_(r)
+    beside = torch.empty_like(r)
+    ws, wsb = workspace(G.OP_DW, x, dz, N, K, M)
+    kw = dict(out_type=G.TYPES["f32"], workspace=ws, workspace_bytes=wsb, stream=stream())
+    G.linear_dw(0, G.TYPES["bf16"], x, dz, beside, N, K, M, residual=r, **kw)
+    G.linear_dw(0, G.TYPES["bf16"], x, dz, dw, N, K, M, residual=dw, lddw=M + pad, ldr=M + pad, **kw)
+    G.sync(0, stream())
+    assert bool(torch.equal(dw.isnan(), beside.isnan()))
+    assert bool(torch.equal(dw.nan_to_num(nan=0.0), beside.nan_to_num(nan=0.0)))
+    dw.fill_(7.0)
+    assert bool((buf == 7.0).all()), "an element between rows was written"
+
+
+@pytest.mark.gpu
 def test_dw_long_sum_in_32_bits(gemm):
     # accumulated over many rows, the f32 gradient stays within 1e-6 of the 64-bit sum (2-norm): partial sums of
     # 512 rows leave the tensor cores, whose adds cut, before 512/16 of them have lost 32 * 2^-25 = 1e-6
