@@ -100,14 +100,14 @@ Plan plan(const LinearArgs& a) {
   Plan best = {0, 1};
   const bool f32 = a.out_type == kTypeF32;
   const int num_kb = (a.depth + kKb - 1) / kKb;
-  // f32 sums leave TMEM every kSegment blocks (dw 2048 x 4096 x 11008: 167 us against 147)
-  double t = pair_time(a) * (f32 && num_kb > kSegment ? 1.15 : 1.0);
+  // f32 sums leave TMEM every 8 blocks (dw 2048 x 4096 x 11008: 167 us against 147)
+  double t = pair_time(a) * (f32 && num_kb > segment_blocks(kTypeF32) ? 1.15 : 1.0);
   for (int bn = a.op == kOpDw ? 64 : 16; bn <= 256; bn *= 2) {
     const long tiles = (long)((a.rows + bn - 1) / bn) * ((a.cols + 127) / 128);
     if (16L * bn < a.rows) continue;   // the fit's range: up to 16 row tiles, 4 CTAs per SM where split
     for (int S = 1; S <= std::min({kMaxSplit, num_kb, bn == 256 ? 4 : kMaxSplit}); ++S) {
       if (S > 1 && tiles * S > 4L * a.num_sms) break;
-      if (f32 && (num_kb + S - 1) / S > kSegment * split_segments(bn)) continue;
+      if ((num_kb + S - 1) / S > split_blocks(bn, a.out_type)) continue;
       const double u = split_time(a, bn, S);
       if (u < t) t = u, best = {bn, S};
     }

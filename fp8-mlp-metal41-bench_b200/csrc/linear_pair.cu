@@ -16,11 +16,10 @@ namespace {
 // 35 instructions per element (2048 x 512 x 11008 with gelu, dropout and residual: 50 us,
 // with eight warps 55), and because 64 columns per thread leave room for f32 sums.
 //
-// F32 results (dW alone): the tensor cores cut low bits when they add to an
-// accumulator, about 2^-25 of it per step of 16, which grows with the contraction
-// (measured against 64 bits: 6e-7 after 512, 5e-6 after 4096).  So every 512 deep the
-// partial sum leaves TMEM and is added in registers, rounded to nearest.  16-bit results,
-// whose own rounding is 2^-12 or 2^-9, keep one accumulation.
+// Partial sums (segment_blocks) leave TMEM while the next one is computed in the other
+// accumulator, and are added in registers.  With f32 results (dW alone) the tile is
+// finished from there; with 16-bit results the sum goes back over the last accumulator,
+// because an epilogue with an activation needs the registers.
 //
 // Bound by the tensor cores, and over a run of such calls by the board's power: linear
 // 2048 x 4096 x 11008 bf16 147 us, 1250 TFLOP/s (76 % of the measured burst, 90 % of the
@@ -169,7 +168,9 @@ __device__ __forceinline__ void tile_out(unsigned char* st, bool tma, const CUte
   }
 }
 
-template <int OP, int TYPE, bool F32, int ACT>
+// DEEP: 16-bit results of more than one partial sum (what that needs in registers would cost
+// the others 0.3 to 1.5 %)
+template <int OP, int TYPE, bool F32, int ACT, bool DEEP>
 __global__ void __launch_bounds__(kPairThreads, 1)
     linear_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                        const __grid_constant__ CUtensorMap tmOut, const __grid_constant__ CUtensorMap tmRes,
@@ -183,7 +184,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   const uint32_t rank = cluster_ctarank();
   const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
   const int num_tiles = p.tiles_r * p.tiles_c;
-  const int seg = F32 ? kSegment : p.num_kb;
+  constexpr int seg = segment_blocks(F32 ? (int)kTypeF32 : TYPE);
   AbortCtl ctl{p.e.dev_err, &bars->abort_flag};
 
   if (threadIdx.x == 0) {
@@ -284,21 +285,26 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         tc_fence_after();
         return ok;
       };
+      // adds the partial sum that comes next and hands its accumulator back
+      auto drain = [&](float (&sum)[64]) {
+        const int buf = local & 1;
+        if (!acquire(buf)) return false;
+#pragma unroll
+        for (int j = 0; j < 64; j += 16) {
+          uint32_t ra[16];
+          tmem_ld_32x32b_x16(quad + (uint32_t)(buf * C::BN + j), ra);
+          tmem_ld_wait();
+          if (j == 48) release(buf);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sum[j + i] += __uint_as_float(ra[i]);
+        }
+        ++local;
+        return true;
+      };
       if constexpr (F32) {
         float sum[64] = {};
-        for (int s0 = 0; s0 < p.num_kb; s0 += seg, ++local) {
-          const int buf = local & 1;
-          if (!acquire(buf)) break;
-#pragma unroll
-          for (int j = 0; j < 64; j += 16) {
-            uint32_t ra[16];
-            tmem_ld_32x32b_x16(quad + (uint32_t)(buf * C::BN + j), ra);
-            tmem_ld_wait();
-            if (j == 48) release(buf);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) sum[j + i] += __uint_as_float(ra[i]);
-          }
-        }
+        for (int s0 = 0; s0 < p.num_kb; s0 += seg)
+          if (!drain(sum)) break;
         if (!ok) break;
         // two staged tiles of 32 columns
 #pragma unroll
@@ -320,8 +326,26 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           tile_out(st.buf, p.out_tma, &tmOut, p.e.out, p.e.ldo, 4, row0, cg, p.e.rows, p.e.cols);
         }
       } else {
+        if constexpr (DEEP) {
+          float sum[64] = {};
+          for (int s0 = 0; s0 + seg < p.num_kb; s0 += seg)
+            if (!drain(sum)) break;
+          if (!ok || !acquire(local & 1)) break;
+          const uint32_t last = quad + (uint32_t)((local & 1) * C::BN);
+#pragma unroll
+          for (int j = 0; j < 64; j += 16) {
+            uint32_t ra[16];
+            tmem_ld_32x32b_x16(last + (uint32_t)j, ra);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) ra[i] = __float_as_uint(sum[j + i] + __uint_as_float(ra[i]));
+            tmem_st_32x32b_x16(last + (uint32_t)j, ra);
+          }
+          tmem_st_wait();
+        } else if (!acquire(local & 1)) {
+          break;
+        }
         const int buf = local & 1;
-        if (!acquire(buf)) break;
         ++local;
         const uint32_t acc = quad + (uint32_t)(buf * C::BN);
         if (!live) {
@@ -402,8 +426,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   }
 }
 
-template <int OP, int TYPE, bool F32, int ACT>
-cudaError_t launch_one(const LinearArgs& a, const Operand& x, const Operand& y) {
+template <int OP, int TYPE, bool F32, int ACT, bool DEEP>
+cudaError_t launch_kernel(const LinearArgs& a, const Operand& x, const Operand& y) {
   using C = PairCfg<OP>;
   PairArgs p = {};
   p.e = epilogue(a);
@@ -438,13 +462,20 @@ cudaError_t launch_one(const LinearArgs& a, const Operand& x, const Operand& y) 
   cfg.numAttrs = 2;
   static Once once;
   int pairs = 0;
-  auto k = linear_pair_kernel<OP, TYPE, F32, ACT>;
+  auto k = linear_pair_kernel<OP, TYPE, F32, ACT, DEEP>;
   cudaError_t e = prepare(once, k, C::SMEM, cfg, &pairs);
   if (e != cudaSuccess) return e;
   if (pairs <= 0) return cudaErrorInvalidConfiguration;
   pairs = std::min(pairs, p.tiles_r * p.tiles_c);
   cfg.gridDim = dim3(2 * pairs);
   return cudaLaunchKernelEx(&cfg, k, tmA, tmB, tmO, tmR, tmZ, p);
+}
+
+template <int OP, int TYPE, bool F32, int ACT>
+cudaError_t launch_one(const LinearArgs& a, const Operand& x, const Operand& y) {
+  if constexpr (!F32)
+    if (a.depth > segment_blocks(TYPE) * kKb) return launch_kernel<OP, TYPE, F32, ACT, true>(a, x, y);
+  return launch_kernel<OP, TYPE, F32, ACT, false>(a, x, y);
 }
 
 template <int TYPE>

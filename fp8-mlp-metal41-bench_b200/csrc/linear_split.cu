@@ -18,12 +18,11 @@ namespace {
 // weights with the launch and the sums in it; 13 x 11008 x 4096 17.5 us.  From 64 rows on by
 // what an SM reads from L2 (about 100 GB/s): 256 x 4096 x 4096 15.4 us.
 //
-// f32 results (dW): the contraction is cut into partial sums of kSegment blocks here too,
-// side by side in TMEM and added with rounding when they are read out (8192 x 1024 x 1024:
-// 32.6 us, the pair kernel 47 us).
+// A CTA's partial sums lie side by side in TMEM and are added with rounding when they are
+// read out (dW 8192 x 1024 x 1024 in f32: 32.6 us, the pair kernel 47 us).
 constexpr int kSplitThreads = 256;
 
-template <int OP, int BN, bool F32>
+template <int OP, int BN, bool DEEP>
 struct SplitCfg {
   static constexpr bool C_MN = OP != kOpDx, R_MN = OP == kOpDw;
   static constexpr int C_BYTES = 128 * 128, R_BYTES = BN * 128;
@@ -34,12 +33,13 @@ struct SplitCfg {
   static constexpr int PER_SM = BN <= 128 ? 2 : 1;
   static constexpr int BAR_OFF = STAGES * STAGE_BYTES;
   static constexpr int SMEM = BAR_OFF + 512 + 1024;
-  static constexpr int SEGS = F32 ? split_segments(BN) : 1;   // accumulators, kSegment blocks each
-  static constexpr uint32_t TMEM_COLS = BN < 32 ? 32 : SEGS * BN;
+  static constexpr int SEGS = DEEP ? split_segments(BN) : 1;   // accumulators
+  static constexpr uint32_t TMEM_COLS = BN < 32 && !DEEP ? 32 : SEGS * BN;
   static constexpr uint32_t IDESC = (1u << 4) | ((C_MN ? 1u : 0u) << 15) | ((R_MN ? 1u : 0u) << 16) |
                                     ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
   static_assert(BN * 512 <= BAR_OFF, "partial sums fit the ring");
   static_assert(SMEM * PER_SM <= kSmemMax, "shared memory budget");
+  static_assert(TMEM_COLS * PER_SM <= 512, "TMEM budget");
   static_assert(!R_MN || BN % 64 == 0, "whole MN boxes");
 };
 
@@ -74,11 +74,13 @@ __device__ __forceinline__ uint32_t cluster_nctarank() {
   return r;
 }
 
-template <int OP, int TYPE, int BN, bool F32>
-__global__ void __launch_bounds__(kSplitThreads, SplitCfg<OP, BN, F32>::PER_SM)
+// DEEP: several partial sums per CTA (where one will do, the code that adds them costs 2 to 3 %
+// all the same: dx 256 x 1024 x 1024 5.24 against 5.08 us)
+template <int OP, int TYPE, int BN, bool F32, bool DEEP>
+__global__ void __launch_bounds__(kSplitThreads, SplitCfg<OP, BN, DEEP>::PER_SM)
     linear_split_kernel(const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmR,
                         const __grid_constant__ EpiArgs p) {
-  using C = SplitCfg<OP, BN, F32>;
+  using C = SplitCfg<OP, BN, DEEP>;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -91,6 +93,8 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<OP, BN, F32>::PER_SM)
   const int num_kb = (p.depth + kKb - 1) / kKb;
   // this CTA's run of the contraction; not empty, S <= num_kb (<= 2^24: 32 bits hold the products)
   const int kb0 = num_kb * rank / S, kb1 = num_kb * (rank + 1) / S;
+  // blocks per partial sum; no more of them than SEGS, the caller sees to it
+  constexpr int seg = segment_blocks(F32 ? (int)kTypeF32 : TYPE);
   AbortCtl ctl{p.dev_err, &bars->abort_flag};
 
   auto load_stage = [&](uint32_t stage, int kb) {
@@ -138,17 +142,19 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<OP, BN, F32>::PER_SM)
     const uint32_t smem_base = smem_u32(smem);
     constexpr uint32_t fmt = TYPE == kTypeBF16 ? 1u : 0u;
     const uint32_t idesc = C::IDESC | (fmt << 7) | (fmt << 10);
-    for (int kb = kb0; kb < kb1; ++kb) {
+    uint32_t d = tmem_base;
+    for (int kb = kb0, at = 0; kb < kb1; ++kb, ++at) {
+      if (DEEP && at == seg) {   // a fresh accumulator
+        at = 0;
+        d += BN;
+      }
       if (!mbar_wait(&bars->full[stage], phase, ctl, 0x300 + stage)) { aborted_any = true; break; }
       tc_fence_after();
       const uint32_t a = smem_base + stage * C::STAGE_BYTES, b = a + C::C_BYTES;
-      const int run = kb - kb0;   // f32: a fresh accumulator every kSegment blocks
-      const uint32_t d = F32 ? tmem_base + (uint32_t)(run / kSegment * BN) : tmem_base;
-      const bool fresh = F32 ? run % kSegment == 0 : run == 0;
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk)
         tc_mma<kKindF16>(d, op_desc(a, C::C_MN, kk), op_desc(b, C::R_MN, kk), idesc,
-                         (!fresh || kk != 0) ? 1u : 0u);
+                         (at != 0 || kk != 0) ? 1u : 0u);
       tc_commit(&bars->empty[stage]);
       if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
     }
@@ -168,11 +174,12 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<OP, BN, F32>::PER_SM)
         if constexpr (CH == 16) tmem_ld_32x32b_x16(acc + (uint32_t)n0, r);
         else tmem_ld_32x32b_x32(acc + (uint32_t)n0, r);
         tmem_ld_wait();
-        if constexpr (F32) {   // the other partial sums, added with rounding
+        if constexpr (DEEP) {   // the other partial sums, added with rounding
 #pragma unroll 1
-          for (int g = 1; g * kSegment < kb1 - kb0; ++g) {
+          for (int g = 1; g * seg < kb1 - kb0; ++g) {
             uint32_t x[CH];
-            tmem_ld_32x32b_x32(acc + (uint32_t)(g * BN + n0), x);
+            if constexpr (CH == 16) tmem_ld_32x32b_x16(acc + (uint32_t)(g * BN + n0), x);
+            else tmem_ld_32x32b_x32(acc + (uint32_t)(g * BN + n0), x);
             tmem_ld_wait();
 #pragma unroll
             for (int i = 0; i < CH; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) + __uint_as_float(x[i]));
@@ -274,9 +281,9 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<OP, BN, F32>::PER_SM)
   if (S > 1) cluster_sync_relaxed();
 }
 
-template <int OP, int TYPE, int BN, bool F32 = false>
-cudaError_t launch_one(const LinearArgs& a, const Operand& x, const Operand& y, int S) {
-  using C = SplitCfg<OP, BN, F32>;
+template <int OP, int TYPE, int BN, bool F32, bool DEEP>
+cudaError_t launch_kernel(const LinearArgs& a, const Operand& x, const Operand& y, int S) {
+  using C = SplitCfg<OP, BN, DEEP>;
   const EpiArgs p = epilogue(a);
   CUtensorMap tmC, tmR;
   if (!map_rows(&tmC, y.p, y.ld, y.rows, y.cols, 2, C::C_MN ? kKb : 128) ||
@@ -297,10 +304,18 @@ cudaError_t launch_one(const LinearArgs& a, const Operand& x, const Operand& y, 
   cfg.attrs = attr;
   cfg.numAttrs = 2;
   static Once once;
-  auto k = linear_split_kernel<OP, TYPE, BN, F32>;
+  auto k = linear_split_kernel<OP, TYPE, BN, F32, DEEP>;
   cudaError_t e = prepare(once, k, C::SMEM, cfg, nullptr);
   if (e != cudaSuccess) return e;
   return cudaLaunchKernelEx(&cfg, k, tmC, tmR, p);
+}
+
+template <int OP, int TYPE, int BN, bool F32 = false>
+cudaError_t launch_one(const LinearArgs& a, const Operand& x, const Operand& y, int S) {
+  if constexpr (!F32)
+    if (((a.depth + kKb - 1) / kKb + S - 1) / S <= segment_blocks(TYPE))
+      return launch_kernel<OP, TYPE, BN, F32, false>(a, x, y, S);
+  return launch_kernel<OP, TYPE, BN, F32, true>(a, x, y, S);
 }
 
 template <int OP, int TYPE>

@@ -1,0 +1,92 @@
+"""The MLP layer's operators at the ends of their ranges: long contractions, far values, wide tiles."""
+import math
+
+import pytest
+
+import test_layer as L
+from mlpgemm import lib as G
+from test_layer import _torch  # noqa: F401 - sets test_layer.torch for GPU tests
+
+torch = None
+
+
+@pytest.fixture(autouse=True)
+def _own_torch(request):
+    global torch
+    if request.node.get_closest_marker("gpu"):
+        import torch as t
+        torch = t
+
+
+# ---- long contractions -------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("type,op,N,K,M", [
+    ("f16", "linear", 4200, 131072, 40), ("f16", "linear", 5, 600000, 40), ("f16", "linear", 300, 70000, 264),
+    ("f16", "linear", 4300, 4160, 264), ("f16", "dx", 4200, 40, 131072), ("f16", "dx", 20, 1032, 100000),
+    ("f16", "dw", 1 << 20, 72, 88), ("f16", "dw", 120000, 72, 88), ("f16", "dw", 50001, 264, 24),
+    ("bf16", "linear", 4200, 600000, 24), ("bf16", "dw", 600000, 136, 200), ("bf16", "dx", 9, 40, 300000),
+    ("bf16", "spread", 4200, 600000, 24)])
+def test_16_bit_sums_of_long_contractions(gemm, type, op, N, K, M):
+    # All products are positive, so every bit that the tensor cores cut off makes a result smaller and nothing cancels.
+    # A partial sum is at most 4096 deep for f16 and 32768 for bf16: a step for every 16 and 16 more inside one, each
+    # cutting at most one unit of 2^-23; adding the partial sums rounds to nearest.
+    # "spread" scales X's rows, so that the results lie on all sides of the type's steps.
+    spread, op = op == "spread", "linear" if op == "spread" else op
+    t = L.ttype(type)
+    depth = {"linear": K, "dx": M, "dw": N}[op]
+    deep = 4096 if type == "f16" else 32768
+    g = torch.Generator(device="cuda").manual_seed(7)
+    scale = 2.0 ** -4 if depth < 200000 else 2.0 ** -6
+
+    def positive(*shape):
+        return ((torch.rand(shape, generator=g, device="cuda") + 0.5) * scale).to(t)
+
+    a = positive(*{"linear": (N, K), "dx": (N, M), "dw": (N, K)}[op])
+    b = positive(*{"linear": (K, M), "dx": (K, M), "dw": (N, M)}[op])
+    if spread:
+        a *= torch.linspace(1, 2, N, device="cuda").to(t)[:, None]
+    shape = {"linear": (N, M), "dx": (N, K), "dw": (K, M)}[op]
+    out = torch.full(shape, float("nan"), dtype=t, device="cuda")
+    ws, wsb = L.workspace({"linear": G.OP_LINEAR, "dx": G.OP_DX, "dw": G.OP_DW}[op], a, b, N, K, M)
+    kw = dict(workspace=ws, workspace_bytes=wsb, stream=L.stream())
+    if op == "linear":
+        z = torch.full(shape, float("nan"), dtype=t, device="cuda")
+        G.linear(0, G.TYPES[type], a, b, out, N, K, M, act=G.ACTS["relu"], preact=z, **kw)
+    else:
+        (G.linear_dx if op == "dx" else G.linear_dw)(0, G.TYPES[type], a, b, out, N, K, M, **kw)
+    G.sync(0, L.stream())
+    ref = torch.zeros(shape, dtype=torch.float64, device="cuda")
+    for i in range(0, depth, 32768):
+        s = slice(i, i + 32768)
+        ref += {"linear": lambda: a[:, s].double() @ b[s].double(), "dx": lambda: a[:, s].double() @ b[:, s].double().t(),
+                "dw": lambda: a[s].double().t() @ b[s].double()}[op]()
+    cut = (min(deep, depth) / 16 + 16) * 2.0 ** -23 + (depth / deep + 8) * 2.0 ** -24
+    L.assert_close(out, ref, L.half_step(ref, t) * 1.01 + ref * cut, op)
+    # Over the whole matrix the roundings of the results cancel (five standard deviations of their mean) as far as the
+    # values spread over the type's steps: rounding to steps s is a sawtooth of x, sum over k of (s / pi k) sin(2 pi k x / s)
+    # up to signs, whose mean over normally distributed x of deviation d is at most the sum of (s / pi k)
+    # exp(-2 (pi k d / s)^2) <= (s / pi) q / (1 - q), q = exp(-2 (pi d / s)^2), and never above s / 2
+    off = float(((out.double() - ref) / ref).mean())
+    step = 2.0 ** math.floor(math.log2(float(ref.max()))) * torch.finfo(t).eps
+    q = math.exp(-2 * (math.pi * float(ref.std()) / step) ** 2)
+    shared = min(step / 2, step / math.pi * q / (1 - q)) / float(ref.min())
+    assert abs(off) <= cut + shared + 5 * torch.finfo(t).eps / 2 * ref.numel() ** -0.5, off
+    if op == "linear":
+        assert torch.equal(z, out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type,K", [("f16", 8300), ("bf16", 66000)])
+def test_epilogue_behind_several_partial_sums(gemm, type, K):
+    # the pair kernel's whole epilogue where the sum is put together from three parts
+    N, M, t = 4200, 520, L.ttype(type)
+    x, w, b, r = L.rand((N, K), t, 1), L.rand((K, M), t, 2, K ** -0.5), L.rand((M,), t, 3), L.rand((N, M), t, 4)
+    y, z = torch.empty(N, M, dtype=t, device="cuda"), torch.empty(N, M, dtype=t, device="cuda")
+    ws, wsb = L.workspace(G.OP_LINEAR, x, w, N, K, M)
+    for act in L.ACT_NAMES:
+        G.linear(0, G.TYPES[type], x, w, y, N, K, M, bias=b, act=G.ACTS[act], residual=r, preact=z,
+                 dropout_p=0.2, seed=3, offset=4, workspace=ws, workspace_bytes=wsb, stream=L.stream())
+        G.sync(0, L.stream())
+        ry, rz, ty, tz = L.linear_ref(x, w, b, r, act, 0.2, 3, 4)
+        L.assert_close(y, ry, ty, "Y")
+        L.assert_close(z, rz, tz, "Z")
