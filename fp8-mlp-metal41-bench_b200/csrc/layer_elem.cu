@@ -156,9 +156,8 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(const __grid_constant
 // A cluster's CTAs share the rows of one slab of columns.  Each thread's eight column
 // sums meet the CTA's other rows in shared memory and the other CTAs' over distributed
 // shared memory, always in the same order.
-// 2048 x 11008 bf16 with the sums: 19.2 us without an activation (4.7 TB/s), 29 us with
-// gelu (4.6 TB/s), 35 us with gelu and dropout, where the 36 instructions per element fill
-// 58 % of all issue slots.
+// 2048 x 11008 bf16 with the sums: 19.2 us without an activation (4.7 TB/s), 28 us with
+// gelu (4.9 TB/s), 37 us with gelu and dropout.
 template <int TYPE, int ACT, int THREADS, bool WIDE>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) act_grad_kernel(const __grid_constant__ ActGradArgs p, int lx,
                                                                            int vy, int vz, int vd) {
@@ -234,8 +233,8 @@ struct GradPlan {
 };
 
 // What counts, measured over all pairs of slab width and S at twelve shapes: SMs with equal
-// numbers of CTAs, three or four of 256 threads each (2048 x 11008 with dropout: 34.5 us
-// with 86 slabs x 8, 41.7 us with 86 x 4), four rows per thread (300 x 11008: 7.5 us with
+// numbers of CTAs, three or four of 256 threads each (2048 x 11008 with dropout: 1.2
+// times as long with 86 slabs x 4 as with 86 x 8), four rows per thread (300 x 11008: 7.5 us with
 // 86 x 4, 9.0 us with 86 x 8) and rows of whole 128-byte lines (2048 x 4096: 15.6 us with
 // 64 slabs x 8, 18.3 us with 128 x 8).  Sizes of S between the powers of two never paid
 // (2048 x 11008: 38.2 us with 172 x 6), clusters of 16 for narrow matrices alone (16384 x

@@ -90,3 +90,58 @@ def test_epilogue_behind_several_partial_sums(gemm, type, K):
         ry, rz, ty, tz = L.linear_ref(x, w, b, r, act, 0.2, 3, 4)
         L.assert_close(y, ry, ty, "Y")
         L.assert_close(z, rz, tz, "Z")
+
+
+# ---- activations over their whole range --------------------------------------------------------
+def lower(z, act):
+    """The factor of z in act(z), Phi(z) or a sigmoid, in 64 bits; and the exponent of the exp in it."""
+    if act == "gelu":
+        return 0.5 * torch.special.erfc(-z / 2 ** 0.5), z * z / 2
+    u = (8 / math.pi) ** 0.5 * (z + 0.044715 * z ** 3) if act == "gelu_tanh" else z
+    return torch.sigmoid(u), u
+
+
+def act_and_slope(z, act):
+    """act(z) and act'(z) in 64 bits with the errors that f32 arithmetic brings: 48 roundings and 1.5e-5 of approximation
+    relative to the small side, and five roundings (2^-24) of the exponent, which pass to what falls with it, the small side.
+    The slope's two terms cancel at its one zero.  Where the factor is below 2^-126 it
+    counts as 0; the slope has it times 1 + |z u'| at most."""
+    p, power = lower(z, act)
+    small = lower(-z.abs(), act)[0]
+    if act == "gelu":
+        q = z * torch.exp(-z * z / 2) / (2 * math.pi) ** 0.5
+        d = torch.ones_like(z)
+    else:
+        d = (8 / math.pi) ** 0.5 * (1 + 0.134145 * z * z) if act == "gelu_tanh" else torch.ones_like(z)
+        q = z * p * lower(-z, act)[0] * d
+    c, e = 48 * 2.0 ** -24, 1.5e-5 + 5 * power.abs() * 2.0 ** -24
+    lost = 2.0 ** -126 * (1 + z.abs() * d)
+    return z * p, (c * p + e * small) * z.abs() + lost, p + q, c * (p + q.abs()) + e * (small + q.abs()) + lost
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh"])
+def test_activations_keep_their_digits(gemm, act, type):
+    # every value of the type from 2^-12 to 1000 and its negative: results and slopes of the far negative side are tiny
+    # and have to be as exact, relative to themselves, as any other
+    t = L.ttype(type)
+    bits = torch.arange(1 << 15, dtype=torch.int32, device="cuda").to(torch.int16).view(t)
+    v = bits[(bits >= 2.0 ** -12) & (bits <= 1000)]
+    v = torch.cat([v, -v, torch.zeros(8, dtype=t, device="cuda")])
+    n = v.numel() // 8 * 8
+    v = v[-n:].contiguous()
+    z = v.double()
+    y, ey, s, es = act_and_slope(z, act)
+    one = torch.zeros(8, dtype=t, device="cuda")
+    one[0] = 1
+    for x, w, N, M in ((one[None], torch.stack([v] + [torch.zeros_like(v)] * 7), 1, n),             # a row of them
+                       (v[:, None] * one[None], one[:, None] * torch.ones(8, device="cuda", dtype=t), n, 8)):
+        out = torch.full((N, M), float("nan"), dtype=t, device="cuda")
+        G.linear(0, G.TYPES[type], x, w, out, N, 8, M, act=G.ACTS[act], stream=L.stream())
+        G.sync(0, L.stream())
+        L.assert_close(out[0] if N == 1 else out[:, 0], y, L.half_step(y, t) * 1.01 + ey, act)
+    dy, dz = torch.ones_like(v), torch.full_like(v, float("nan"))
+    G.act_grad(0, G.TYPES[type], dy, v, dz, None, n // 8, 8, act=G.ACTS[act], stream=L.stream())
+    G.sync(0, L.stream())
+    L.assert_close(dz, s, L.half_step(s, t) * 1.01 + es, act + "'")
