@@ -226,8 +226,8 @@ __device__ __forceinline__ void act_fwd_n(float (&v)[W], int act) {
 }
 
 // act'(z).  z is a stored pre-activation, which f16 may have rounded to an
-// infinity: beyond the clamps every slope is 0 or 1 to f32 precision, so an
-// infinite z gets its limit instead of inf * 0.  NaN stays NaN.
+// infinity: beyond the clamps the exps are 0 or infinite in f32 and every slope is 0 or 1,
+// so an infinite z gets its limit instead of inf * 0.  NaN stays NaN.
 template <int ACT>
 __device__ __forceinline__ f32x2 act_slope2(f32x2 z) {
   const f32x2 one = pair2(1.f), minus = pair2(-1.f);
@@ -254,7 +254,7 @@ __device__ __forceinline__ f32x2 act_slope2(f32x2 z) {
     return mul2(q, fma2(d, fma2(q, minus, one), one));
   }
   if constexpr (ACT == kActSilu) {
-    z = clamp2(z, 80.f);
+    z = clamp2(z, 90.f);   // e^-80 = 2e-35 is a bf16 number still
     const f32x2 q = sigmoid2(mul2(z, pair2(-1.4426950408889634f)));
     return mul2(q, fma2(z, fma2(q, minus, one), one));
   }

@@ -121,7 +121,7 @@ def act_and_slope(z, act):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("type", ["f16", "bf16"])
-@pytest.mark.parametrize("act", ["gelu", "gelu_tanh"])
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
 def test_activations_keep_their_digits(gemm, act, type):
     # every value of the type from 2^-12 to 1000 and its negative: results and slopes of the far negative side are tiny
     # and have to be as exact, relative to themselves, as any other
