@@ -415,9 +415,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     while (global_ns() - t0 < 100000ull) {}
   }
   __syncwarp();
-  // Not earlier: the next kernel's CTAs would crowd onto the SMs that the last, partial
-  // round of tiles leaves idle.
-  griddep_launch();
+  // the next kernel may be set up once every CTA has stored its last tile (linear_split.cu)
+  if (warp >= 4) griddep_launch();
   tc_fence_before();
   cluster_sync();
   if (warp == 1) {

@@ -197,7 +197,10 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<OP, BN, DEEP>::PER_SM)
     while (global_ns() - t0 < 100000ull) {}
   }
   __syncwarp();
-  griddep_launch();   // not earlier: the next kernel's CTAs would fill this one's gaps unevenly
+  // The next kernel may be set up once every CTA's partial sums are in shared memory; the first
+  // thread of a CTA counts for all, so warps without a part in the sums don't ask.  Asked for
+  // right after the set-up, calls take the same time to 1 %; not at all, 1 us more.
+  if (warp >= 4) griddep_launch();
   if (S > 1) cluster_sync();
   else __syncthreads();
   if (warp == 1) {
