@@ -794,7 +794,9 @@ extern "C" {
 
 size_t gemm_linear_workspace(int op, const void* A, long lda, const void* B, long ldb, int N, int K, int M) {
   if (op < kOpLinear || op > kOpDw || !dim_ok(N) || !dim_ok(K) || !dim_ok(M) || !A || !B) return 0;
-  return linear_workspace(product(op, A, lda, B, ldb, N, K, M));
+  const LinearArgs a = product(op, A, lda, B, ldb, N, K, M);
+  if (!elem_aligned(A, kTypeF16) || !elem_aligned(B, kTypeF16) || a.lda < (op == kOpDx ? M : K) || a.ldb < M) return 0;
+  return linear_workspace(a);
 }
 
 int gemm_linear(int device, int type, const void* X, long ldx, const void* W, long ldw, void* Y, long ldy, int N,
