@@ -6,6 +6,7 @@ or cannot be loaded, every entry point here raises GemmError.
 from __future__ import annotations
 
 import ctypes
+import operator
 import os
 import struct
 import subprocess
@@ -387,12 +388,97 @@ def quantize(device, fmt, src, dst, scales=None, rows=1, cols=1, stream=None) ->
 
 
 # ---- the MLP layer (f16 / bf16 operands; see the header for the formulas) -----------------
-def _dropout(p, seed, offset, offset_ptr) -> bytes:
-    return DROPOUT_ARGS.pack(p, seed & _U64, offset & _U64, as_ptr(offset_ptr) or 0)
+# What the C side can't see of a torch tensor or DeviceBuffer is checked here: a host tensor, another
+# GPU's, or one that is smaller or laid out otherwise than the call takes it for would have the kernels
+# read or write where they must not.
+_dtypes = {}    # GEMM_TYPE_* -> torch dtype, once a torch tensor has been seen
+_layer = {}     # the entry points without argtypes, whose conversion takes 0.1 us per argument:
+                # pointers, longs and sizes go in as ctypes objects, the rest are ints of 32 bits
+
+_VP, _LONG, _SIZE = ctypes.c_void_p, ctypes.c_long, ctypes.c_size_t
+_LONG0, _SIZE0 = _LONG(0), _SIZE(0)
+
+
+def _refuse(name: str, why: str):
+    raise GemmError(GEMM_ERR_ARGS, f"{name} {why}")
+
+
+def _bind(name):
+    fn = _layer[name] = lib()[name]
+    return fn
+
+
+def _ints(*values):
+    """The same as Python's own ints, which ctypes would cut to 32 bits without a word."""
+    values = [operator.index(v) for v in values]
+    for v in values:
+        if not -(1 << 31) <= v < 1 << 31:
+            _refuse(f"size {v}", "does not fit an int")
+    return values
+
+
+def _on(device, name, x):
+    """Address of a buffer on `device`."""
+    if x is None or x.__class__ is int:
+        return x
+    if hasattr(x, "get_device"):
+        if x.get_device() != device:
+            _refuse(name, f"is on {x.device}, not on device {device}")
+        return x.data_ptr()
+    if isinstance(x, DeviceBuffer) and x.device != device:
+        _refuse(name, f"is on device {x.device}, not on device {device}")
+    return as_ptr(x)
+
+
+def _matrix(x, dtype, device, type, rows, cols, ld, name):
+    """Address of rows x cols elements of `type` (torch's `dtype`), `ld` from row to row (0: dense)."""
+    if x is None or x.__class__ is int:
+        return x
+    try:   # the usual case
+        if (x.dtype is dtype and x.get_device() == device and x.is_contiguous()
+                and x.numel() >= (rows - 1) * (ld or cols) + cols):
+            return x.data_ptr()
+    except AttributeError:
+        pass
+    need = (rows - 1) * (ld or cols) + cols
+    if hasattr(x, "get_device"):
+        if not _dtypes:
+            import torch
+            _dtypes.update({TYPES["f16"]: torch.float16, TYPES["bf16"]: torch.bfloat16, TYPES["f32"]: torch.float32})
+        if x.dtype is not _dtypes.get(type):
+            _refuse(name, f"has elements of {x.dtype}, not of type {type}")
+        if x.is_contiguous():
+            if x.numel() < need:
+                _refuse(name, f"has {x.numel()} elements, {need} needed")
+        elif x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1) or x.stride(0) != (ld or cols):
+            _refuse(name, f"of strides {tuple(x.stride())} does not have rows {ld or cols} elements apart")
+        elif x.shape[0] < rows or x.shape[1] < cols:
+            _refuse(name, f"is {tuple(x.shape)}, {rows} x {cols} needed")
+    elif isinstance(x, DeviceBuffer) and x.nbytes < need * (4 if type == TYPES["f32"] else 2):
+        _refuse(name, f"has {x.nbytes} bytes, {need} elements needed")
+    return _on(device, name, x)
+
+
+def _scratch(device, x, nbytes):
+    """Workspace address and bytes as the C side takes them."""
+    if x is None and not nbytes:
+        return None, _SIZE0
+    if hasattr(x, "get_device"):
+        have = x.numel() * x.element_size()
+    else:
+        have = x.nbytes if isinstance(x, DeviceBuffer) else nbytes
+    if have < nbytes:
+        _refuse("workspace", f"has {have} bytes, {nbytes} given")
+    return _VP(_on(device, "workspace", x)), _SIZE(int(nbytes))
+
+
+def _dropout(device, p, seed, offset, offset_ptr) -> bytes:
+    return DROPOUT_ARGS.pack(p, seed & _U64, offset & _U64, _on(device, "offset_ptr", offset_ptr) or 0)
 
 
 def linear_workspace(op: int, A, B, N: int, K: int, M: int, lda: int = 0, ldb: int = 0) -> int:
     """Workspace bytes of a product: A, B are X, W (OP_LINEAR), dZ, W (OP_DX) or X, dZ (OP_DW)."""
+    N, K, M = _ints(N, K, M)
     return lib().gemm_linear_workspace(op, as_ptr(A), lda, as_ptr(B), ldb, N, K, M)
 
 
@@ -400,40 +486,90 @@ def linear(device, type, X, W, Y, N, K, M, bias=None, act=0, residual=None, prea
            offset=0, offset_ptr=None, ldx=0, ldw=0, ldy=0, ldr=0, ldz=0, workspace=None, workspace_bytes=0,
            stream=None) -> None:
     """Y = residual + dropout(act(X @ W + bias)); preact receives X @ W + bias.  Row lengths 0: dense."""
-    epi = EPILOGUE.pack(as_ptr(bias) or 0, as_ptr(residual) or 0, ldr, as_ptr(preact) or 0, ldz, act, dropout_p,
-                        seed & _U64, offset & _U64, as_ptr(offset_ptr) or 0)
-    check(lib().gemm_linear(device, type, as_ptr(X), ldx, as_ptr(W), ldw, as_ptr(Y), ldy, N, K, M,
-                            epi, as_ptr(workspace), int(workspace_bytes), as_ptr(stream)),
-          "gemm_linear")
+    all_ = N | K | M | device | type
+    if all_.__class__ is not int or all_ >> 31:
+        device, type, N, K, M = _ints(device, type, N, K, M)
+    dt = _dtypes.get(type)
+    ws, wsb = _scratch(device, workspace, workspace_bytes)
+    epi = EPILOGUE.pack(_matrix(bias, dt, device, type, 1, M, 0, "bias") or 0,
+                        _matrix(residual, dt, device, type, N, M, ldr, "residual") or 0, ldr,
+                        _matrix(preact, dt, device, type, N, M, ldz, "preact") or 0, ldz, act, dropout_p,
+                        seed & _U64, offset & _U64, _on(device, "offset_ptr", offset_ptr) or 0)
+    rc = (_layer.get("gemm_linear") or _bind("gemm_linear"))(
+        device, type, _VP(_matrix(X, dt, device, type, N, K, ldx, "X")), _LONG(ldx) if ldx else _LONG0,
+        _VP(_matrix(W, dt, device, type, K, M, ldw, "W")), _LONG(ldw) if ldw else _LONG0,
+        _VP(_matrix(Y, dt, device, type, N, M, ldy, "Y")), _LONG(ldy) if ldy else _LONG0, N, K, M, epi, ws, wsb,
+        _VP(as_ptr(stream)))
+    if rc:
+        check(rc, "gemm_linear")
 
 
 def linear_dx(device, type, dZ, W, dX, N, K, M, residual=None, lddz=0, ldw=0, lddx=0, ldr=0, workspace=None,
               workspace_bytes=0, stream=None) -> None:
     """dX = residual + dZ @ W^T."""
-    check(lib().gemm_linear_dx(device, type, as_ptr(dZ), lddz, as_ptr(W), ldw, as_ptr(dX), lddx, N, K, M,
-                               as_ptr(residual), ldr, as_ptr(workspace), int(workspace_bytes), as_ptr(stream)),
-          "gemm_linear_dx")
+    all_ = N | K | M | device | type
+    if all_.__class__ is not int or all_ >> 31:
+        device, type, N, K, M = _ints(device, type, N, K, M)
+    dt = _dtypes.get(type)
+    ws, wsb = _scratch(device, workspace, workspace_bytes)
+    rc = (_layer.get("gemm_linear_dx") or _bind("gemm_linear_dx"))(
+        device, type, _VP(_matrix(dZ, dt, device, type, N, M, lddz, "dZ")), _LONG(lddz) if lddz else _LONG0,
+        _VP(_matrix(W, dt, device, type, K, M, ldw, "W")), _LONG(ldw) if ldw else _LONG0,
+        _VP(_matrix(dX, dt, device, type, N, K, lddx, "dX")), _LONG(lddx) if lddx else _LONG0, N, K, M,
+        _VP(_matrix(residual, dt, device, type, N, K, ldr, "residual")), _LONG(ldr) if ldr else _LONG0, ws, wsb,
+        _VP(as_ptr(stream)))
+    if rc:
+        check(rc, "gemm_linear_dx")
 
 
 def linear_dw(device, type, X, dZ, dW, N, K, M, out_type=None, residual=None, ldx=0, lddz=0, lddw=0, ldr=0,
               workspace=None, workspace_bytes=0, stream=None) -> None:
     """dW = residual + X^T @ dZ, of `out_type` (default: the operands' type)."""
-    check(lib().gemm_linear_dw(device, type, as_ptr(X), ldx, as_ptr(dZ), lddz, as_ptr(dW),
-                               type if out_type is None else out_type, lddw, N, K, M, as_ptr(residual), ldr,
-                               as_ptr(workspace), int(workspace_bytes), as_ptr(stream)), "gemm_linear_dw")
+    out = type if out_type is None else out_type
+    all_ = N | K | M | device | type | out
+    if all_.__class__ is not int or all_ >> 31:
+        device, type, out, N, K, M = _ints(device, type, out, N, K, M)
+    dt, dto = _dtypes.get(type), _dtypes.get(out)
+    ws, wsb = _scratch(device, workspace, workspace_bytes)
+    rc = (_layer.get("gemm_linear_dw") or _bind("gemm_linear_dw"))(
+        device, type, _VP(_matrix(X, dt, device, type, N, K, ldx, "X")), _LONG(ldx) if ldx else _LONG0,
+        _VP(_matrix(dZ, dt, device, type, N, M, lddz, "dZ")), _LONG(lddz) if lddz else _LONG0,
+        _VP(_matrix(dW, dto, device, out, K, M, lddw, "dW")), out, _LONG(lddw) if lddw else _LONG0, N, K, M,
+        _VP(_matrix(residual, dto, device, out, K, M, ldr, "residual")), _LONG(ldr) if ldr else _LONG0, ws, wsb,
+        _VP(as_ptr(stream)))
+    if rc:
+        check(rc, "gemm_linear_dw")
 
 
 def act_grad(device, type, dY, Z, dZ, dbias, N, M, act=0, dropout_p=0.0, seed=0, offset=0, offset_ptr=None,
              lddy=0, ldz=0, lddz=0, stream=None) -> None:
     """dZ = dropout(dY) * act'(Z); dbias (f32) = its column sums."""
-    drop = _dropout(dropout_p, seed, offset, offset_ptr)
-    check(lib().gemm_act_grad(device, type, as_ptr(dY), lddy, as_ptr(Z), ldz, as_ptr(dZ), lddz, as_ptr(dbias), N, M,
-                              act, drop, as_ptr(stream)), "gemm_act_grad")
+    all_ = N | M | device | type | act
+    if all_.__class__ is not int or all_ >> 31:
+        device, type, act, N, M = _ints(device, type, act, N, M)
+    dt = _dtypes.get(type)
+    drop = _dropout(device, dropout_p, seed, offset, offset_ptr)
+    rc = (_layer.get("gemm_act_grad") or _bind("gemm_act_grad"))(
+        device, type, _VP(_matrix(dY, dt, device, type, N, M, lddy, "dY")), _LONG(lddy) if lddy else _LONG0,
+        _VP(_matrix(Z, dt, device, type, N, M, ldz, "Z")), _LONG(ldz) if ldz else _LONG0,
+        _VP(_matrix(dZ, dt, device, type, N, M, lddz, "dZ")), _LONG(lddz) if lddz else _LONG0,
+        _VP(_matrix(dbias, _dtypes.get(2), device, 2, 1, M, 0, "dbias")), N, M, act, drop, _VP(as_ptr(stream)))
+    if rc:
+        check(rc, "gemm_act_grad")
 
 
 def dropout(device, type, X, Y, N, M, p, seed, offset, offset_ptr=None, residual=None, ldx=0, ldr=0, ldy=0,
             stream=None) -> None:
     """Y = residual + dropout(X); on dY the same call is its gradient."""
-    drop = _dropout(p, seed, offset, offset_ptr)
-    check(lib().gemm_dropout(device, type, as_ptr(X), ldx, as_ptr(residual), ldr, as_ptr(Y), ldy, N, M,
-                             drop, as_ptr(stream)), "gemm_dropout")
+    all_ = N | M | device | type
+    if all_.__class__ is not int or all_ >> 31:
+        device, type, N, M = _ints(device, type, N, M)
+    dt = _dtypes.get(type)
+    drop = _dropout(device, p, seed, offset, offset_ptr)
+    rc = (_layer.get("gemm_dropout") or _bind("gemm_dropout"))(
+        device, type, _VP(_matrix(X, dt, device, type, N, M, ldx, "X")), _LONG(ldx) if ldx else _LONG0,
+        _VP(_matrix(residual, dt, device, type, N, M, ldr, "residual")), _LONG(ldr) if ldr else _LONG0,
+        _VP(_matrix(Y, dt, device, type, N, M, ldy, "Y")), _LONG(ldy) if ldy else _LONG0, N, M, drop,
+        _VP(as_ptr(stream)))
+    if rc:
+        check(rc, "gemm_dropout")
