@@ -719,6 +719,14 @@ int check_matrix(const char* name, const void* p, int type, long ld, int cols, b
   return GEMM_OK;
 }
 
+// A result in an input's own buffer has that input's row length: a row must not be written
+// where another one is still to be read.
+int check_in_place(const char* on, const void* out, long ldo, const char* in, const void* p, long ld, int rows) {
+  if (out && out == p && rows > 1 && ldo != ld)
+    return fail(GEMM_ERR_ARGS, "%s in %s's buffer with rows %ld apart, not %ld", on, in, ldo, ld);
+  return GEMM_OK;
+}
+
 int make_dropout(const gemm_dropout_args* in, DropArgs* out) {
   *out = DropArgs();
   if (!in) return GEMM_OK;
@@ -772,6 +780,7 @@ int run_product(int device, LinearArgs& a, int type, int out_type, const char* a
   a.ldo = dense(ldo, a.cols);
   a.res = res;
   a.ldr = dense(ldr, a.cols);
+  if ((rc = check_in_place(on, out, a.ldo, "residual", res, a.ldr, a.rows))) return rc;
   a.ws = ws;
   a.ws_bytes = ws_bytes;
   const size_t need = linear_workspace(a);
@@ -809,8 +818,9 @@ int gemm_linear(int device, int type, const void* X, long ldx, const void* W, lo
   if ((rc = make_dropout(&q.dropout, &a.drop))) return rc;
   if (q.bias && !elem_aligned(q.bias, type)) return fail(GEMM_ERR_ARGS, "bias is not aligned to its element");
   if ((rc = check_matrix("preact", q.preact, type, q.ldz, M, true))) return rc;
-  if (q.preact && (q.preact == Y || q.preact == X || q.preact == W || q.preact == q.residual))
+  if (q.preact && (q.preact == Y || q.preact == X || q.preact == W || q.preact == q.residual || q.preact == q.bias))
     return fail(GEMM_ERR_ARGS, "preact and another operand are the same buffer");
+  if (q.bias && q.bias == Y) return fail(GEMM_ERR_ARGS, "Y and bias are the same buffer");
   a.bias = q.bias;
   a.pre = q.preact;
   a.ldz = dense(q.ldz, M);
@@ -859,6 +869,8 @@ int gemm_act_grad(int device, int type, const void* dY, long lddy, const void* Z
   a.lddy = dense(lddy, M);
   a.ldz = dense(ldz, M);
   a.lddz = dense(lddz, M);
+  if ((rc = check_in_place("dZ", dZ, a.lddz, "dY", dY, a.lddy, N))) return rc;
+  if ((rc = check_in_place("dZ", dZ, a.lddz, "Z", act == kActNone ? nullptr : Z, a.ldz, N))) return rc;
   DevState* s = dev_state(device);
   if (!s) return fail(GEMM_ERR_INIT, "device %d not initialised (call gemm_init)", device);
   a.stream = static_cast<cudaStream_t>(stream);
@@ -889,6 +901,8 @@ int gemm_dropout(int device, int type, const void* X, long ldx, const void* resi
   a.ldx = dense(ldx, M);
   a.ldr = dense(ldr, M);
   a.ldy = dense(ldy, M);
+  if ((rc = check_in_place("Y", Y, a.ldy, "X", X, a.ldx, N))) return rc;
+  if ((rc = check_in_place("Y", Y, a.ldy, "residual", residual, a.ldr, N))) return rc;
   DevState* s = dev_state(device);
   if (!s) return fail(GEMM_ERR_INIT, "device %d not initialised (call gemm_init)", device);
   a.stream = static_cast<cudaStream_t>(stream);

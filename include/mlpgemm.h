@@ -319,7 +319,8 @@ int gemm_quantize(int device, int format, const float *src, void *dst, void *sca
  * graph gets new masks from replay to replay by writing it in between.
  *
  * R (`residual`) has the result's type and may be the result's buffer itself (the
- * same pointer and row length); no other input may overlap an output.  Elements
+ * same pointer and row length, another one is refused); no other input may overlap
+ * an output.  Elements
  * between a row's end and the next row are neither read nor written.
  * N, K, M are 1 .. 2^30.  Pointers are aligned to their element.  Any size,
  * stride and alignment works; X, W and dZ are read in place where their base and

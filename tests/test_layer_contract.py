@@ -106,3 +106,28 @@ def test_sizes_of_other_integer_types():
     passes("linear_dw", N=i(N), out_type=i(1))
     passes("act_grad", N=i(N), act=i(1))
     passes("dropout", M=i(M), seed=5, offset=7)
+
+
+# ---- results in an input's buffer --------------------------------------------------------------
+def in_place(kw_of, *words):
+    """kw_of(ld of the result, rows): refused where the input's rows are 80 apart and the result's are not."""
+    refused(lambda: kw_of(96, 4), *words)
+    refused(lambda: kw_of(0, 2), *words)
+    for ld, rows in ((80, 4), (96, 1), (0, 1)):        # the same rows, or a single one
+        with pytest.raises(G.GemmError) as e:
+            kw_of(ld, rows)
+        assert e.value.code == G.GEMM_ERR_INIT, e.value
+
+
+def test_results_in_place_have_the_inputs_rows():
+    Q, R = P + (1 << 16), P + (2 << 16)
+    in_place(lambda ld, n: G.linear(-1, 0, P, Q, R, n, 64, 72, residual=R, ldr=80, ldy=ld), "Y", "residual")
+    in_place(lambda ld, n: G.linear_dx(-1, 0, P, Q, R, n, 72, 64, residual=R, ldr=80, lddx=ld), "dX", "residual")
+    in_place(lambda ld, k: G.linear_dw(-1, 0, P, Q, R, 64, 8 * (k > 1) or 1, 72, out_type=2, residual=R, ldr=80, lddw=ld,
+                                       ldx=8), "dW", "residual")
+    in_place(lambda ld, n: G.act_grad(-1, 0, P, Q, P, None, n, 72, act=2, lddy=80, lddz=ld), "dZ", "dY")
+    in_place(lambda ld, n: G.act_grad(-1, 0, P, Q, Q, None, n, 72, act=2, ldz=80, lddz=ld), "dZ", "Z's buffer")
+    in_place(lambda ld, n: G.dropout(-1, 0, P, P, n, 72, 0.5, 1, 2, ldx=80, ldy=ld), "Y", "X")
+    in_place(lambda ld, n: G.dropout(-1, 0, P, Q, n, 72, 0.5, 1, 2, residual=Q, ldr=80, ldy=ld), "Y", "residual")
+    refused(lambda: G.linear(-1, 0, P, Q, R, 4, 64, 72, bias=R), "bias", "same buffer")
+    refused(lambda: G.linear(-1, 0, P, Q, R, 4, 64, 72, bias=R + 4096, preact=R + 4096), "preact", "same buffer")
