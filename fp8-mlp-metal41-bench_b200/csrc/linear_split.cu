@@ -40,6 +40,8 @@ struct SplitCfg {
   static_assert(BN * 512 <= BAR_OFF, "partial sums fit the ring");
   static_assert(SMEM * PER_SM <= kSmemMax, "shared memory budget");
   static_assert(TMEM_COLS * PER_SM <= 512, "TMEM budget");
+  static_assert(SMEM > 228 * 1024 - 160 * 1024, "no room beside the peak probe (peak.cu)");
+  static_assert((PER_SM + 1) * SMEM > 228 * 1024, "no third CTA on an SM, so none waits for TMEM");
   static_assert(!R_MN || BN % 64 == 0, "whole MN boxes");
 };
 

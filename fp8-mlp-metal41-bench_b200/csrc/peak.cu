@@ -38,7 +38,12 @@ constexpr int kA = 128 * 128;             // A tile bytes (128 rows x 128 B)
 constexpr int kB = kPeakN * 128;          // B tile bytes (256 rows x 128 B)
 constexpr int kSfOff = kA + kB;           // 512 B of unit scale factors
 constexpr int kBarOff = kSfOff + 512;
-constexpr int kPeakSmem = kBarOff + 64 + 1024;
+// More than the probe uses: it takes all of TMEM, and CTAs of two clusters that share two SMs
+// and wait there for each other's TMEM would wait for good.  The other kernels with TMEM that
+// run as clusters (the GEMM's pairs, the layer's products) need 92 KB at least, so that none
+// fits beside this.
+constexpr int kPeakSmem = 160 * 1024;
+static_assert(kPeakSmem >= kBarOff + 64 + 1024, "tiles");
 
 template <int KIND, bool PAIR, bool BMN = false>
 constexpr uint32_t peak_idesc() {
