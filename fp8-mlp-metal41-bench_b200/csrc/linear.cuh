@@ -9,7 +9,8 @@
 //   linear_pair.cu    persistent, 256 x 256 tiles on CTA pairs, for many tiles
 //   linear_split.cu   128 columns x BN rows per CTA, the contraction split over a
 //                     cluster: few rows, where the weights' bytes bound the call
-//   linear.cu         the choice between them; operands that the TMA cannot read
+//   linear_plan.h     the choice between them
+//   linear.cu         operands that the TMA cannot read
 //
 // Every mbarrier wait is bounded (ptx.cuh); on expiry a kernel records an error
 // word, lets its TMA copies land, frees TMEM and returns.  No load uses multicast.
@@ -21,25 +22,14 @@
 #include <mutex>
 
 #include "layer.cuh"
+#include "linear_plan.h"
 #include "ptx.cuh"
 #include "tmap.h"
 
 namespace mlpg {
 
-constexpr int kKb = 64;            // contraction elements per stage: one 128-byte swizzle row
 constexpr int kBoxBytes = 64 * 128;   // one MN-major box: 64 contraction rows x 64 elements
 constexpr int kSmemMax = 232448;
-constexpr int kMaxSplit = 8;       // portable cluster size
-
-// The tensor cores cut low bits when they add to an accumulator: on average about 2^-25 of
-// it per step of 16, at most 2^-23, always towards zero, so the loss grows with the
-// contraction (2-norm against 64 bits: 6e-7 after 512, 5e-6 after 4096).  The contraction is
-// therefore cut into partial sums that start from zero and are added in f32, rounded to
-// nearest.  Blocks per partial sum at most: 512 deep for f32 results; for 16-bit ones as much
-// as keeps the loss below 1/15 of half a step of the type, 4096 deep for f16 and 32768 for
-// bf16.  (2048 x 11008 x 4096 with a residual: 144.6 us with a single sum, 147.9 us every
-// 4096, 149.7 us every 1024.)
-constexpr int segment_blocks(int out_type) { return out_type == kTypeF32 ? 8 : (out_type == kTypeF16 ? 64 : 512); }
 
 struct EpiArgs {
   const void *bias, *res;
@@ -142,10 +132,6 @@ cudaError_t prepare(Once& once, Kernel k, int smem, cudaLaunchConfig_t& cfg, int
 // rows_op, cols_op: the stored operands whose rows or columns index the result's rows
 // and columns (A and B of LinearArgs, packed where they had to be)
 cudaError_t launch_pair(const LinearArgs& a, const Operand& rows_op, const Operand& cols_op);
-// The split kernel's partial sums per CTA, which fill its share of TMEM, and the blocks of the
-// contraction that they hold
-constexpr int split_segments(int bn) { return bn == 256 ? 2 : 256 / bn; }
-constexpr int split_blocks(int bn, int out_type) { return segment_blocks(out_type) * split_segments(bn); }
 // bn rows per CTA (16, 32, 64, 128, 256; dW from 64), clusters of `split`; at most split_blocks
 // blocks of the contraction per CTA
 cudaError_t launch_split(const LinearArgs& a, const Operand& rows_op, const Operand& cols_op, int bn, int split);

@@ -18,6 +18,54 @@ def _own_torch(request):
         torch = t
 
 
+# ---- every kernel ---------------------------------------------------------------------------------
+# (op, type, type of the result, N, K, M): what the shapes of test_layer.py do not reach (test_layer_plan.py checks)
+KERNELS = [
+    ("dx", "f16", "f16", 2136, 616, 7656), ("dx", "bf16", "bf16", 2101, 24, 4192), ("dx", "f16", "f16", 2061, 24, 696),
+    ("dw", "bf16", "f32", 4625, 1, 24), ("dw", "bf16", "f32", 4489, 1035, 24), ("dw", "bf16", "f32", 1186, 3888, 313),
+    ("dw", "f16", "f32", 4269, 65, 40), ("dw", "f16", "f32", 4520, 1056, 24), ("dw", "f16", "f32", 2080, 2184, 24),
+    # contractions of several partial sums per CTA
+    ("linear", "f16", "f16", 4156, 4416, 24), ("linear", "f16", "f16", 1, 32808, 24), ("linear", "f16", "f16", 137, 33632, 136),
+    ("linear", "f16", "f16", 529, 35272, 24), ("linear", "f16", "f16", 1063, 35136, 24), ("linear", "f16", "f16", 2140, 16944, 24),
+    ("linear", "bf16", "bf16", 4165, 33328, 24), ("linear", "bf16", "bf16", 1, 262872, 24),
+    ("linear", "bf16", "bf16", 135, 268376, 136), ("linear", "bf16", "bf16", 532, 268793, 24),
+    ("linear", "bf16", "bf16", 1032, 262224, 24), ("linear", "bf16", "bf16", 2063, 131344, 24),
+    ("dx", "f16", "f16", 4336, 24, 4296), ("dx", "f16", "f16", 1, 24, 33176), ("dx", "f16", "f16", 129, 136, 37369),
+    ("dx", "f16", "f16", 517, 24, 35424), ("dx", "f16", "f16", 1040, 24, 33552), ("dx", "f16", "f16", 2109, 24, 16608),
+    ("dx", "bf16", "bf16", 4315, 24, 39032), ("dx", "bf16", "bf16", 1, 24, 263256), ("dx", "bf16", "bf16", 264, 24, 266456),
+    ("dx", "bf16", "bf16", 522, 24, 279248), ("dx", "bf16", "bf16", 1100, 24, 266136), ("dx", "bf16", "bf16", 2106, 24, 136968),
+    ("dw", "f16", "f16", 131699, 1, 24), ("dw", "f16", "f16", 48034, 1, 24), ("dw", "f16", "f16", 33008, 1088, 24),
+    ("dw", "f16", "f16", 16760, 2072, 24), ("dw", "bf16", "bf16", 1087830, 1, 136), ("dw", "bf16", "bf16", 268775, 1, 24),
+    ("dw", "bf16", "bf16", 283912, 1032, 24), ("dw", "bf16", "bf16", 164943, 2096, 24)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", KERNELS, ids=str)
+def test_every_kernel(gemm, case):
+    # with a residual, in the result's own buffer and beside it: the same bits
+    op, type, out, N, K, M = case
+    t, o = L.ttype(type), L.ttype(out)
+    a = L.rand(*{"linear": ((N, K), t, 1), "dx": ((N, M), t, 1), "dw": ((N, K), t, 1)}[op])
+    b = L.rand(*{"linear": ((K, M), t, 2), "dx": ((K, M), t, 2), "dw": ((N, M), t, 2)}[op], scale=0.125)
+    r = L.rand({"linear": (N, M), "dx": (N, K), "dw": (K, M)}[op], o, 3)
+    kind, call = {"linear": (G.OP_LINEAR, G.linear), "dx": (G.OP_DX, G.linear_dx), "dw": (G.OP_DW, G.linear_dw)}[op]
+    ws, wsb = L.workspace(kind, a, b, N, K, M)
+    kw = dict(workspace=ws, workspace_bytes=wsb, stream=L.stream())
+    if op == "dw":
+        kw["out_type"] = G.TYPES[out]
+    y, same = torch.full_like(r, float("nan")), r.clone()
+    call(0, G.TYPES[type], a, b, y, N, K, M, residual=r, **kw)
+    call(0, G.TYPES[type], a, b, same, N, K, M, residual=same, **kw)
+    G.sync(0, L.stream())
+    a, b = {"linear": lambda: (a, b), "dx": lambda: (a, b.t()), "dw": lambda: (a.t(), b)}[op]()
+    depth, deep = a.shape[1], {"f16": 4096, "bf16": 32768, "f32": 512}[out]
+    v = a.double() @ b.double() + r.double()
+    # the cut of one partial sum (one unit of 2^-23 per step), and the additions of all
+    e = (a.double().abs() @ b.double().abs()) * ((min(depth, deep) / 16 + 16) * 2.0 ** -23 + (depth / deep + 8) * 2.0 ** -24)
+    L.assert_close(y, v, e + v.abs() * 2.0 ** -23 + L.half_step(v, o) * 1.01, op)
+    assert torch.equal(same, y)
+
+
 # ---- long contractions -------------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("type,op,N,K,M", [
