@@ -27,6 +27,10 @@ int row_unit(const void* p, long ld) {
 }
 
 constexpr int kDepth = 4;
+// act_grad adds the values of a thread's rows one by one.  Where there are more rows than this,
+// each such run starts from zero and then joins the others: the roundings of equal values go
+// the same way (a column of 270001 of them was 2e-5 off with 2100 in one run).
+constexpr int kRun = 128;
 
 // A thread's walk down its rows of one operand: the next row's address, and the unit in
 // which its eight columns are read or written (2 for a group that ends behind the row).
@@ -158,10 +162,12 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(const __grid_constant
 // shared memory, always in the same order.
 // 2048 x 11008 bf16 with the sums: 19.2 us without an activation (4.7 TB/s), 28 us with
 // gelu (4.9 TB/s), 37 us with gelu and dropout.
-template <int TYPE, int ACT, int THREADS, bool WIDE>
+// LONG: several runs per thread (in one kernel with the rest, that rest takes 1 to 4 % longer).
+template <int TYPE, int ACT, int THREADS, bool WIDE, bool LONG>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) act_grad_kernel(const __grid_constant__ ActGradArgs p, int lx,
                                                                            int vy, int vz, int vd) {
-  extern __shared__ uint4 ring[];                 // kDepth rows of one or two operands
+  constexpr int kOps = ACT == kActNone ? 1 : 2;
+  extern __shared__ uint4 ring[];                 // kDepth rows of one or two operands, LONG: and the runs' sums
   float* part = reinterpret_cast<float*>(ring);   // the sums, once the ring is drained
   const int t = (int)threadIdx.x, ty = THREADS >> lx, tx = 1 << lx;
   const int S = (int)gridDim.y, rank = (int)blockIdx.y;   // the cluster is the grid's y
@@ -170,27 +176,46 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) act_grad_kernel(const
   griddep_wait();
   if (c < p.M) {
     const uint64_t off = drop_offset(p.drop);
-    const int rows = S * ty, r = rank * ty + (t >> lx);
+    const int rows = S * ty;
+    int r = rank * ty + (t >> lx);
     Walk d = walk(p.dZ, p.lddz, vd, r, rows, c, p.M);
-    stream_rows<THREADS, ACT == kActNone ? 1 : 2, WIDE>(smem_u32(ring + t), walk(p.dY, p.lddy, vy, r, rows, c, p.M),
-                                         walk(p.Z, p.ldz, vz, r, rows, c, p.M), r, rows, p.N, c, p.M,
-                                         [&](int row, auto first, auto second) {
-      const uint4 b = p.drop.on ? drop_bits(p.drop, off, row, g) : make_uint4(0, 0, 0, 0);
-      float v[8];
-      unpack8<TYPE>(v, first());
-      if constexpr (ACT != kActNone) {
-        float w[8];
-        unpack8<TYPE>(w, second());
+    auto run = [&](int end) {
+      stream_rows<THREADS, kOps, WIDE>(smem_u32(ring + t), walk(p.dY, p.lddy, vy, r, rows, c, p.M),
+                                       walk(p.Z, p.ldz, vz, r, rows, c, p.M), r, rows, end, c, p.M,
+                                       [&](int row, auto first, auto second) {
+        const uint4 b = p.drop.on ? drop_bits(p.drop, off, row, g) : make_uint4(0, 0, 0, 0);
+        float v[8];
+        unpack8<TYPE>(v, first());
+        if constexpr (ACT != kActNone) {
+          float w[8];
+          unpack8<TYPE>(w, second());
+#pragma unroll
+          for (int j = 0; j < 8; j += 2)
+            split2(mul2(pair2(v[j], v[j + 1]), act_slope2<ACT>(pair2(w[j], w[j + 1]))), v[j], v[j + 1]);
+        }
+        if (p.drop.on) drop8(v, p.drop, b);
+        if (p.dZ) put8<TYPE, WIDE>(v, d, c, p.M);
 #pragma unroll
         for (int j = 0; j < 8; j += 2)
-          split2(mul2(pair2(v[j], v[j + 1]), act_slope2<ACT>(pair2(w[j], w[j + 1]))), v[j], v[j + 1]);
-      }
-      if (p.drop.on) drop8(v, p.drop, b);
-      if (p.dZ) put8<TYPE, WIDE>(v, d, c, p.M);
+          split2(add2(pair2(sum[j], sum[j + 1]), pair2(v[j], v[j + 1])), sum[j], sum[j + 1]);
+      });
+    };
+    if constexpr (LONG) {
+      float4* total = reinterpret_cast<float4*>(ring + kDepth * kOps * THREADS) + 2 * t;
+      total[0] = total[1] = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (; r < p.N; r += kRun * rows) {
+        run(p.N - r > kRun * rows ? r + kRun * rows : p.N);
+        const float4 x = total[0], y = total[1];
+        total[0] = make_float4(x.x + sum[0], x.y + sum[1], x.z + sum[2], x.w + sum[3]);
+        total[1] = make_float4(y.x + sum[4], y.y + sum[5], y.z + sum[6], y.w + sum[7]);
 #pragma unroll
-      for (int j = 0; j < 8; j += 2)
-        split2(add2(pair2(sum[j], sum[j + 1]), pair2(v[j], v[j + 1])), sum[j], sum[j + 1]);
-    });
+        for (int j = 0; j < 8; ++j) sum[j] = 0.f;
+      }
+      const float4 x = total[0], y = total[1];
+      sum[0] = x.x, sum[1] = x.y, sum[2] = x.z, sum[3] = x.w, sum[4] = y.x, sum[5] = y.y, sum[6] = y.z, sum[7] = y.w;
+    } else {
+      run(p.N);
+    }
   }
   griddep_launch();
   if (!p.dbias) return;   // the same for the whole cluster
@@ -271,10 +296,11 @@ GradPlan grad_plan(const ActGradArgs& a) {
   return best;
 }
 
-template <int TYPE, int ACT, int THREADS, bool WIDE>
-cudaError_t launch_act_grad_typed(const ActGradArgs& a, const GradPlan& pl) {
-  auto kernel = act_grad_kernel<TYPE, ACT, THREADS, WIDE>;
-  constexpr int smem = kDepth * (ACT == kActNone ? 1 : 2) * THREADS * 16;   // at least the sums' 32 bytes a thread
+template <int TYPE, int ACT, int THREADS, bool WIDE, bool LONG>
+cudaError_t launch_act_grad_kernel(const ActGradArgs& a, const GradPlan& pl) {
+  auto kernel = act_grad_kernel<TYPE, ACT, THREADS, WIDE, LONG>;
+  // the rings; at least, and LONG besides, the sums' 32 bytes a thread
+  constexpr int smem = (kDepth * (ACT == kActNone ? 1 : 2) * 16 + (LONG ? 32 : 0)) * THREADS;
   static_assert(smem >= THREADS * 32, "sums");
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
@@ -297,6 +323,13 @@ cudaError_t launch_act_grad_typed(const ActGradArgs& a, const GradPlan& pl) {
   if (e != cudaSuccess) return e;
   return cudaLaunchKernelEx(&cfg, kernel, a, pl.lx, row_unit(a.dY, a.lddy), row_unit(a.Z, a.ldz),
                             row_unit(a.dZ, a.lddz));
+}
+
+template <int TYPE, int ACT, int THREADS, bool WIDE>
+cudaError_t launch_act_grad_typed(const ActGradArgs& a, const GradPlan& pl) {
+  if (a.dbias && a.N > (long)kRun * pl.S * (THREADS >> pl.lx))
+    return launch_act_grad_kernel<TYPE, ACT, THREADS, WIDE, true>(a, pl);
+  return launch_act_grad_kernel<TYPE, ACT, THREADS, WIDE, false>(a, pl);
 }
 
 template <int TYPE, int ACT>

@@ -193,3 +193,36 @@ def test_activations_keep_their_digits(gemm, act, type):
     G.act_grad(0, G.TYPES[type], dy, v, dz, None, n // 8, 8, act=G.ACTS[act], stream=L.stream())
     G.sync(0, L.stream())
     L.assert_close(dz, s, L.half_step(s, t) * 1.01 + es, act + "'")
+
+
+# ---- column sums of many rows --------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,M", [(270001, 8200), (1000003, 2051), (2000001, 24), (40000, 11008), (20000, 1000)])
+def test_column_sums_of_many_rows(gemm, N, M):
+    t = torch.bfloat16
+    dy = torch.empty(N, M, dtype=t, device="cuda")
+    z, dz, db = torch.empty_like(dy), torch.empty_like(dy), torch.full((M,), float("nan"), device="cuda")
+    # positive values: the roundings of the additions (2^-24 each, 128 rows and then the runs one after the other) are
+    # independent, so over all columns the 2-norm stays far below 1e-6
+    for i in range(0, N, 50000):
+        dy[i:i + 50000] = L.rand((min(50000, N - i), M), t, i + 1).abs()
+        z[i:i + 50000] = L.rand((min(50000, N - i), M), t, i + 2)
+    G.act_grad(0, 1, dy, z, dz, db, N, M, act=G.ACTS["relu"], stream=L.stream())
+    G.sync(0, L.stream())
+    ref = torch.zeros(M, dtype=torch.float64, device="cuda")
+    for i in range(0, N, 50000):
+        v = torch.where(z[i:i + 50000] > 0, dy[i:i + 50000], torch.zeros_like(dy[i:i + 50000]))
+        assert torch.equal(dz[i:i + 50000], v)
+        ref += v.double().sum(0)
+    assert float((db.double() - ref).norm() / ref.norm()) <= 1e-6
+    # equal values: the roundings go the same way; at most 128 rows, the runs (a slab's CTAs take 64 rows at a time or
+    # more), and 8 + 8 + 16 additions that join threads and CTAs
+    dy.fill_(0.1)
+    row = torch.empty(M, device="cuda")
+    for v in (0.3, 0.9, 1.3, 1.7, -0.4):
+        z.fill_(v)
+        G.act_grad(0, 1, dy, z, None, db, N, M, act=G.ACTS["gelu"], stream=L.stream())
+        G.act_grad(0, 1, dy, z, None, row, 1, M, act=G.ACTS["gelu"], stream=L.stream())
+        G.sync(0, L.stream())
+        ref = row.double() * N
+        assert float(((db.double() - ref) / ref).abs().max()) <= (128 + N / (128 * 64) + 32) * 2.0 ** -24, v
