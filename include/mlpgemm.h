@@ -293,8 +293,8 @@ int gemm_quantize(int device, int format, const float *src, void *dst, void *sca
  * else at least the row's length).  Sums are f32 and each result is rounded once,
  * to nearest even.  The tensor cores cut bits when they add, so a product's sum is
  * put together from partial sums with rounded additions: what is cut stays below
- * 1/15 of the result's half step (f16, bf16) and near 1e-6 of the sum (f32; 2-norm)
- * for any length of the contraction.
+ * 1/15 of the result's half step (f16, bf16), and an f32 dW is within 1e-6 (2-norm)
+ * up to a million rows.
  *
  *   gemm_linear     Y[N,M]  = R + D(act(X[N,K] @ W[K,M] + bias))
  *                   Z[N,M]  = X @ W + bias, stored where `preact` is given

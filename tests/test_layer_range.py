@@ -124,6 +124,20 @@ def test_16_bit_sums_of_long_contractions(gemm, type, op, N, K, M):
 
 
 @pytest.mark.gpu
+def test_f32_dw_of_a_million_rows(gemm):
+    # 2048 partial sums of 512 rows.  What each loses, some 5e-7 of it, has random signs and comes to as much of the sum.
+    # An addition rounds off 0.29 units of the last place (root mean square), 0.29 * 0.72 * 2^-23 of a running sum that
+    # grows with the root of its terms: sqrt(2048 / 2) times that is 8e-7.  Both together: 9.4e-7
+    N, K, M = 1 << 20, 136, 88
+    x, dz = L.rand((N, K), torch.bfloat16, 1), L.rand((N, M), torch.bfloat16, 2)
+    dw = torch.empty(K, M, device="cuda")
+    G.linear_dw(0, 1, x, dz, dw, N, K, M, out_type=G.TYPES["f32"], stream=L.stream())
+    G.sync(0, L.stream())
+    ref = x.double().t() @ dz.double()
+    assert float((dw.double() - ref).norm() / ref.norm()) <= 1e-6
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("type,K", [("f16", 8300), ("bf16", 66000)])
 def test_epilogue_behind_several_partial_sums(gemm, type, K):
     # the pair kernel's whole epilogue where the sum is put together from three parts
