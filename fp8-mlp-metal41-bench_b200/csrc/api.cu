@@ -782,7 +782,6 @@ int run_product(int device, LinearArgs& a, int type, int out_type, const char* a
   a.ldr = dense(ldr, a.cols);
   if ((rc = check_in_place(on, out, a.ldo, "residual", res, a.ldr, a.rows))) return rc;
   a.ws = ws;
-  a.ws_bytes = ws_bytes;
   const size_t need = linear_workspace(a);
   if (need && (!ws || ws_bytes < need)) return fail(GEMM_ERR_ARGS, "workspace of %zu bytes required", need);
   if (need && (reinterpret_cast<uintptr_t>(ws) & 15u)) return fail(GEMM_ERR_ARGS, "workspace is not 16-byte aligned");

@@ -116,8 +116,7 @@ struct LinearArgs {
   long ldz;
   int act;
   DropArgs drop;
-  void* ws;
-  size_t ws_bytes;
+  void* ws;                // at least linear_workspace bytes
   cudaStream_t stream;
   int* dev_err;
   int num_sms;

@@ -61,7 +61,7 @@ __device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
 }
 
 // W (4 or 8) elements of a row of `cols` from column c on, element `at` of base: one
-// access where the rows allow it (vec); elements past the row read as 0 and are not written.
+// access where the rows allow it (vec); elements past the row read as 0.
 template <int TYPE, int W>
 __device__ __forceinline__ void loadn(float (&v)[W], const void* base, size_t at, int c, int cols, bool vec) {
   const uint16_t* p = static_cast<const uint16_t*>(base) + at;
@@ -79,15 +79,15 @@ __device__ __forceinline__ void loadn(float (&v)[W], const void* base, size_t at
   }
 }
 
-template <int TYPE, int W>
-__device__ __forceinline__ void storen(const float (&v)[W], void* base, size_t at, int c, int cols, bool vec) {
+// Four elements the same way; none past the row is written.
+template <int TYPE>
+__device__ __forceinline__ void store4(const float (&v)[4], void* base, size_t at, int c, int cols, bool vec) {
   uint16_t* p = static_cast<uint16_t*>(base) + at;
-  if (vec && c + W <= cols) {
-    if constexpr (W == 8) *reinterpret_cast<uint4*>(p) = pack8<TYPE>(v);
-    else *reinterpret_cast<uint2*>(p) = make_uint2(pack2<TYPE>(v[0], v[1]), pack2<TYPE>(v[2], v[3]));
+  if (vec && c + 4 <= cols) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(pack2<TYPE>(v[0], v[1]), pack2<TYPE>(v[2], v[3]));
   } else {
 #pragma unroll
-    for (int i = 0; i < W; ++i)
+    for (int i = 0; i < 4; ++i)
       if (c + i < cols) store1<TYPE>(p, i, v[i]);
   }
 }

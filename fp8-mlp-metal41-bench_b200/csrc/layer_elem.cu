@@ -2,10 +2,10 @@
 // epilogue (with the bias gradient's column sums) and dropout.
 //
 // One pass over the data, eight neighbouring columns (16 bytes) per thread and row.
-// The threads of a CTA form 2^lx column groups x 256 / 2^lx rows, so no index needs a
-// division.  Each thread walks down its rows behind a ring of its own in shared memory
-// that cp.async keeps kDepth - 1 rows ahead: the loads need no registers and no barrier,
-// and the arithmetic of one row runs under the loads of the next ones.
+// A CTA's 256 or 1024 threads form 2^lx column groups by as many rows as that leaves, so no
+// index needs a division.  Each thread walks down its rows behind a ring of its own in
+// shared memory that cp.async keeps kDepth - 1 rows ahead: the loads need no registers and
+// no barrier, and the arithmetic of one row runs under the loads of the next ones.
 #include <cuda_runtime.h>
 
 #include <algorithm>

@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<OP, BN, DEEP>::PER_SM)
 #pragma unroll
           for (int j = 0; j < 4; ++j) v[j] += b[j];
         }
-        if (p.pre) storen<TYPE, 4>(v, p.pre, (size_t)row * p.ldz + c, c, p.cols, p.pre_vec);
+        if (p.pre) store4<TYPE>(v, p.pre, (size_t)row * p.ldz + c, c, p.cols, p.pre_vec);
         act_fwd_n(v, p.act);
         if (p.drop.on) drop4(v, p.drop, off, row, c);
       }
@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(kSplitThreads, SplitCfg<OP, BN, DEEP>::PER_SM)
 #pragma unroll
           for (int j = 0; j < 4; ++j) v[j] += r[j];
         }
-        storen<TYPE, 4>(v, p.out, oa, c, p.cols, p.out_vec);
+        store4<TYPE>(v, p.out, oa, c, p.cols, p.out_vec);
       }
     }
   }
