@@ -38,12 +38,17 @@ cudaError_t pack(Operand& o, unsigned char*& ws, const LinearArgs& a) {
   if (!bytes) return cudaSuccess;
   const int groups = (o.cols + 7) / 8;
   const long grid = std::min(((long)o.rows * groups + 255) / 256, 16L * a.num_sms);
-  pack_rows_kernel<<<(unsigned)grid, 256, 0, a.stream>>>(static_cast<const uint16_t*>(o.p), o.ld,
-                                                         reinterpret_cast<uint16_t*>(ws), o.rows, o.cols, groups);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(256);
+  cfg.stream = a.stream;
+  // the launch's own status: cudaGetLastError would answer with another call's
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, pack_rows_kernel, static_cast<const uint16_t*>(o.p), o.ld,
+                                           reinterpret_cast<uint16_t*>(ws), o.rows, o.cols, groups);
   o.p = ws;
   o.ld = 8L * groups;
   ws += bytes;
-  return cudaGetLastError();
+  return e;
 }
 
 }  // namespace

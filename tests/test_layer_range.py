@@ -240,3 +240,19 @@ def test_column_sums_of_many_rows(gemm, N, M):
         G.sync(0, L.stream())
         ref = row.double() * N
         assert float(((db.double() - ref) / ref).abs().max()) <= (128 + N / (128 * 64) + 32) * 2.0 ** -24, v
+
+
+# ---- errors of other calls ----------------------------------------------------------------------
+@pytest.mark.gpu
+def test_an_earlier_calls_error_is_not_this_ones(gemm):
+    # an allocation that the GPU cannot give fails by itself; the next call, here one that packs its operands, does not
+    with pytest.raises(G.GemmError):
+        G.DeviceBuffer(0, 1 << 50)
+    N, K, M, t = 5, 33, 41, torch.float16
+    x, w, y = L.rand((N, K), t, 1), L.rand((K, M), t, 2), torch.empty(N, M, dtype=t, device="cuda")
+    ws, wsb = L.workspace(G.OP_LINEAR, x, w, N, K, M)
+    assert wsb > 0
+    G.linear(0, 0, x, w, y, N, K, M, workspace=ws, workspace_bytes=wsb, stream=L.stream())
+    G.sync(0, L.stream())
+    ry, _, ty, _ = L.linear_ref(x, w, None, None, "none", 0, 0, 0)
+    L.assert_close(y, ry, ty, "Y")
