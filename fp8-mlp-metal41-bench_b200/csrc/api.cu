@@ -36,6 +36,8 @@ int fail(int code, const char* fmt, ...) {
   vsnprintf(buf, sizeof buf, fmt, ap);
   va_end(ap);
   g_err = buf;
+  // the error is reported: it must not answer a later launch's cudaGetLastError as well
+  if (code != GEMM_ERR_ARGS) (void)cudaGetLastError();
   return code;
 }
 
@@ -351,7 +353,10 @@ int gemm_d2h(int device, void* dst, const void* src, size_t bytes) {
 
 void* gemm_host_alloc(size_t bytes) {
   void* p = nullptr;
-  if (cudaMallocHost(&p, bytes ? bytes : 1) != cudaSuccess) return nullptr;
+  if (cudaMallocHost(&p, bytes ? bytes : 1) != cudaSuccess) {
+    (void)cudaGetLastError();   // reported by the null pointer, as in fail()
+    return nullptr;
+  }
   return p;
 }
 

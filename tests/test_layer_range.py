@@ -256,3 +256,16 @@ def test_an_earlier_calls_error_is_not_this_ones(gemm):
     G.sync(0, L.stream())
     ry, _, ty, _ = L.linear_ref(x, w, None, None, "none", 0, 0, 0)
     L.assert_close(y, ry, ty, "Y")
+
+
+@pytest.mark.gpu
+def test_a_reported_error_is_over(gemm):
+    # the same for the entry points that were there before: they ask cudaGetLastError after their launches
+    src = torch.randn(64, 64, device="cuda")
+    dst = torch.empty(64, 64, dtype=torch.uint8, device="cuda")
+    with pytest.raises(G.GemmError):
+        G.DeviceBuffer(0, 1 << 50)
+    G.quantize(0, G.Q_E4M3, src, dst, None, 64, 64, stream=L.stream())
+    G.sync(0, L.stream())
+    back = dst.view(torch.float8_e4m3fn).double()
+    assert bool(((back - src.double()).abs() <= src.double().abs() * 2.0 ** -4 + 2.0 ** -10).all())
