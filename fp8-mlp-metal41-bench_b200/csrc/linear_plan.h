@@ -20,7 +20,6 @@ constexpr int kMaxSplit = 8;       // portable cluster size
 // 4096, 149.7 us every 1024.)
 constexpr int segment_blocks(int out_type) { return out_type == kTypeF32 ? 8 : (out_type == kTypeF16 ? 64 : 512); }
 
-
 // The split kernel's partial sums per CTA, which fill its share of TMEM, and the blocks of the
 // contraction that they hold
 constexpr int split_segments(int bn) { return bn == 256 ? 2 : 256 / bn; }
